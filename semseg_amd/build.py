@@ -11,7 +11,10 @@ SOURCES = ["conv_igemm.hip", "conv_wgrad.hip", "stem.hip", "bn.hip", "pool_inter
            "psa_ops.hip", "infer.hip", "optim.hip", "augment.hip", "winograd.hip", "gemm_bf16split.hip", "xchg.hip", "plan.hip"]
 HEADER = os.path.join(HERE, "..", "include", "semseg_hip.h")
 THUNKS = os.path.join(CSRC, "plan_thunks.inc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-fPIC", "-shared"]
+# -packed-fp32-ops: no v_pk_add / mul / fma_f32 — some of their forms have given wrong results on this hardware now and then, with no
+# error (hipcc's host pass warns that it does not know the feature: harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-munsafe-fp-atomics", "-fPIC", "-shared",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 OBJ_DIR = os.path.join(CSRC, "build")          # git-ignored; objects are an incremental-build cache only
@@ -83,8 +86,15 @@ def gen_thunks():
     return True
 
 
+def _tag(defines=()):
+    """Of the flags and defines an object was compiled with: part of its cached name."""
+    import hashlib
+    h = hashlib.sha1(" ".join(FLAGS + sorted(defines)).encode()).hexdigest()[:8]
+    return h if defines else "base-" + h
+
+
 def _linked_sources():
-    """Names of the sources the library on disk was linked from (written next to it at link time)."""
+    """The flags' tag and the names of the sources the library on disk was linked from (written next to it at link time)."""
     try:
         return open(LIB + ".sources").read().split()
     except OSError:
@@ -92,7 +102,7 @@ def _linked_sources():
 
 
 def needs_build():
-    if not os.path.exists(LIB) or _linked_sources() != [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]:
+    if not os.path.exists(LIB) or _linked_sources() != [_tag()] + [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]:
         return True
     t = os.path.getmtime(LIB)
     return any(os.path.getmtime(d) > t for s in SOURCES for d in _deps(s) if os.path.exists(d))
@@ -106,11 +116,10 @@ def build(force=False, verbose=False, defines=(), out=None):
     gen_thunks()      # before the staleness check: a header edit changes plan_thunks.inc, which plan.hip includes
     if not force and not defines and out == LIB and not needs_build():
         return LIB
-    import hashlib
     from concurrent.futures import ThreadPoolExecutor
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     os.makedirs(OBJ_DIR, exist_ok=True)
-    tag = hashlib.sha1(" ".join(sorted(defines)).encode()).hexdigest()[:8] if defines else "base"
+    tag = _tag(defines)
     cflags = [f for f in FLAGS if f != "-shared"] + ["-D" + d for d in defines]
     jobs = []
     for src in SOURCES:
@@ -141,7 +150,7 @@ def build(force=False, verbose=False, defines=(), out=None):
         print(" ".join(cmd), file=sys.stderr)
     subprocess.check_call(cmd)
     with open(out + ".sources", "w") as f:
-        f.write("\n".join(j[0] for j in jobs) + "\n")
+        f.write("\n".join([tag] + [j[0] for j in jobs]) + "\n")
     return out
 
 
