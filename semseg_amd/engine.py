@@ -341,11 +341,10 @@ class Engine:
         # (measured bs 16: 217.4 -> 207.9 ms per step together with the high-priority chain below, 214.5 without
         # the side stream; scripts/step_variants.py).
         self.side_all = True
-        # The dependent chain of backward (data gradients + BatchNorm) runs on a high-priority stream so that it wins
-        # the dispatch race against the weight gradients queued on the side stream.
-        # Not under torch.distributed: with the SyncBN all-reduces issued from the high-priority stream the forced
-        # 1-rank RCCL step at batch 2 takes 60.5 ms instead of 39.2 (RCCL's own stream has normal priority and every
-        # collective is an event round trip between the two).
+        # The dependent chain of backward (data gradients + BatchNorm) runs on a stream of its own beside the side stream of the
+        # weight gradients — at the DEFAULT priority: work on streams of different priorities can hang on this hardware.
+        # Not under torch.distributed: with the SyncBN all-reduces issued from a second stream every collective is an event
+        # round trip between the two (forced 1-rank RCCL step at batch 2, then still with a raised priority: 60.5 instead of 39.2 ms).
         self.hipri_main = debug("hipri_main", "1") == "1" and not self.dist_on
         # number of weight-gradient streams used round-robin (each with its own split-K scratch); 2 / 3 / 4 measured
         # slower than 1
@@ -1392,7 +1391,7 @@ class Engine:
         self._f64_zero_sums()
         if self.hipri_main:
             if self._hi is None:
-                self._hi = _shared(self.device, "hipri", lambda: torch.cuda.Stream(device=self.device, priority=-1))
+                self._hi = _shared(self.device, "hipri", lambda: torch.cuda.Stream(device=self.device))
             cur = torch.cuda.current_stream()
             ops.stream_wait(self._hi, cur)
             with torch.cuda.stream(self._hi):
