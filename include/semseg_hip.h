@@ -294,6 +294,58 @@ int semseg_bilinear_bwd(const float* dy, int lddy, float* dx, int lddx, int N, i
 int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int Hi, int Wi, int Ho,
                                  int Wo, int C, hipStream_t stream);
 
+/* ---- class probabilities of logits (no counterpart in the reference): what a model answers with beyond its argmax, and what another
+ * model learns from it.  A row is one pixel (or token) with C logits of type SEMSEG_TYPE_*; row i * p + j (i < n, j < p), class c, is
+ * element i * sn + j * sp + c * sc.  Every [n * p] operand is contiguous in that row order; results and sums are fp32.
+ *
+ * semseg_class_logprobs_fwd: log softmax(z / T) at the row's label (logprob; needs label), its entropy, lse = log sum exp(z / T), and
+ * the k <= SEMSEG_CLASS_TOP_MAX classes of the largest logits with their log probabilities, in falling order, equal logits by rising
+ * class; row (i, j)'s alternative a is element i * tn + j * tp + a * tk of top_ids / top_logprobs.  Any output may be NULL.  stats
+ * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
+ * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
+ * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (the ids stay in range, NaN first).
+ * semseg_class_logprobs_bwd: dz (=|+=) the gradient from those of logprob, entropy, lse (each may be NULL); 0 for rows that are void
+ * or hold only -inf; strides dn, dp, dc; dz has the logits' type, one rounding. */
+enum { SEMSEG_TYPE_F32 = 0, SEMSEG_TYPE_BF16 = 1, SEMSEG_TYPE_F16 = 2 };
+enum { SEMSEG_REDUCE_NONE = 0, SEMSEG_REDUCE_MEAN = 1, SEMSEG_REDUCE_SUM = 2 };
+enum { SEMSEG_CLASS_TOP_MAX = 64 };
+int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
+                              long long sc, const long long* label, long long ignore_index, float T, int k, float* logprob,
+                              float* entropy, float* lse, float* stats, int* top_ids, float* top_logprobs, long long tn,
+                              long long tp, long long tk, hipStream_t stream);
+int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
+                              long long sc, const long long* label, long long ignore_index, float T, const float* stats,
+                              const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_lse,
+                              void* dz, long long dn, long long dp, long long dc, int accumulate, hipStream_t stream);
+/* Distillation from a teacher's k <= SEMSEG_CLASS_TOP_MAX stored classes of every row: ids (int32, or int64 with ids64), values top
+ * (type top_type), element strides in, ip, ik / vn, vp, vk.  A negative id is an absent entry; the same class twice adds up.
+ *   tail = 0: q = softmax(top / T) over the entries present (top: logits, any shift);  loss_r = sum_j q_j (log q_j - log p_{id_j})
+ *   tail = 1: q = exp(top) (log probabilities at T);  + q_rest (log q_rest - log p_rest), the classes outside ids as one class on both
+ *             sides, q_rest = max(0, 1 - sum q); without a finite logit outside ids there is no such class
+ * with p = softmax(z / T).  rows: T^2 * weight_r * loss_r (needed by SEMSEG_REDUCE_NONE, else may be NULL).  loss: their sum (SUM),
+ * over the sum of weights (MEAN; NaN where that is 0, like an all-void cross entropy; gradients 0).  weight NULL: 1; rows of weight 0
+ * are not read.  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
+ * semseg_distill_scratch_bytes() bytes, nothing needs to be cleared; no atomics, results do not depend on scheduling.
+ * _bwd: dz (=|+=) grad_mul * grad_loss (one device float, one per row for NONE, NULL: 1) * d loss / dz.
+ * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call. */
+size_t semseg_distill_scratch_bytes(long long n, long long p, int C);
+int semseg_distill_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp, long long sc,
+                       const void* ids, int ids64, const void* top, int top_type, int k, long long in, long long ip,
+                       long long ik, long long vn, long long vp, long long vk, const float* weight, float T, int tail,
+                       int reduction, float* rows, float* stats, double* acc2, float* loss, void* scratch,
+                       size_t scratch_bytes, hipStream_t stream);
+int semseg_distill_bwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp, long long sc,
+                       const void* ids, int ids64, const void* top, int top_type, int k, long long in, long long ip,
+                       long long ik, long long vn, long long vp, long long vk, const float* weight, float T, int tail,
+                       int reduction, const float* stats, const double* acc2, const float* grad_loss, float grad_mul,
+                       void* dz, long long dn, long long dp, long long dc, int accumulate, hipStream_t stream);
+int semseg_distill_fwd_bwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
+                           long long sc, const void* ids, int ids64, const void* top, int top_type, int k, long long in,
+                           long long ip, long long ik, long long vn, long long vp, long long vk, const float* weight,
+                           float T, int tail, int reduction, float* stats, double* acc2, float* loss, float grad_mul,
+                           void* dz, long long dn, long long dp, long long dc, int accumulate, void* scratch,
+                           size_t scratch_bytes, hipStream_t stream);
+
 /* ---- fused head: upsample + CrossEntropyLoss(ignore_index) + argmax — model/pspnet.py:95,100-103,
  * tool/train.py:121.  acc2 = THREE doubles {sum of losses, valid-pixel count, number of labels that are neither
  * ignore_index nor in [0, C)} (fp64, zeroed by the call), loss = acc2[0]/acc2[1].  Out-of-range labels contribute nothing;

@@ -568,6 +568,62 @@ def ce_head_bwd(scores, ld, label, lse, acc2, grad_loss, grad_mul, dscores, lddz
                                ignore_index, *_scr(scratch), _stream()), "ce_head_bwd")
 
 
+# ---------------------------------------------------------------------------------------------
+# class probabilities: log probabilities, entropy, top alternatives; distillation (semseg_amd.distill is the tensor-level interface)
+# ---------------------------------------------------------------------------------------------
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+def class_logprobs_fwd(z, geom, strides, label, ignore_index, T, k, logprob, entropy, lse, stats, top_ids=None, top_logprobs=None,
+                       top_strides=(0, 0, 0)):
+    """geom (n, p, C), strides (sn, sp, sc): rows i * p + j of z (include/semseg_hip.h); logits of an fp32 / bf16 / fp16 tensor."""
+    _ck(lib.semseg_class_logprobs_fwd(_p(z), TYPES[z.dtype], *geom, *strides, _p(label), int(ignore_index), float(T), k,
+                                      _p(logprob), _p(entropy), _p(lse), _p(stats), _p(top_ids), _p(top_logprobs), *top_strides,
+                                      _stream()), "class_logprobs_fwd")
+
+
+def class_logprobs_bwd(z, geom, strides, label, ignore_index, T, stats, entropy, g_logprob, g_entropy, g_lse, dz, dstrides,
+                       accumulate=False):
+    assert dz.dtype == z.dtype
+    _ck(lib.semseg_class_logprobs_bwd(_p(z), TYPES[z.dtype], *geom, *strides, _p(label), int(ignore_index), float(T), _p(stats),
+                                      _p(entropy), _p(g_logprob), _p(g_entropy), _p(g_lse), _p(dz), *dstrides, int(accumulate),
+                                      _stream()), "class_logprobs_bwd")
+
+
+def distill_scratch_bytes(n, p, C):
+    return int(lib.semseg_distill_scratch_bytes(n, p, C))
+
+
+def _teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction):
+    return (_p(ids), int(ids.dtype == torch.int64), _p(top), TYPES[top.dtype], k, *id_strides, *top_strides, _p(weight), float(T),
+            int(tail), REDUCTIONS[reduction])
+
+
+def distill_fwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, rows, stats, acc2, loss, scratch):
+    _ck(lib.semseg_distill_fwd(_p(z), TYPES[z.dtype], *geom, *strides,
+                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(rows), _p(stats),
+                               _p(acc2), _p(loss), _p(scratch), 0 if scratch is None else scratch.numel() * scratch.element_size(),
+                               _stream()), "distill_fwd")
+
+
+def distill_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, stats, acc2, grad_loss, grad_mul,
+                dz, dstrides, accumulate=False):
+    assert dz.dtype == z.dtype
+    _ck(lib.semseg_distill_bwd(_p(z), TYPES[z.dtype], *geom, *strides,
+                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(stats), _p(acc2),
+                               _p(grad_loss), float(grad_mul), _p(dz), *dstrides, int(accumulate), _stream()), "distill_bwd")
+
+
+def distill_fwd_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, stats, acc2, loss, grad_mul,
+                    dz, dstrides, accumulate, scratch):
+    assert dz.dtype == z.dtype
+    _ck(lib.semseg_distill_fwd_bwd(_p(z), TYPES[z.dtype], *geom, *strides,
+                                   *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(stats), _p(acc2),
+                                   _p(loss), float(grad_mul), _p(dz), *dstrides, int(accumulate), _p(scratch),
+                                   scratch.numel() * scratch.element_size(), _stream()), "distill_fwd_bwd")
+
+
 def dropout2d_mask(mask, p, seed, offset, offset_dev=None):
     """offset_dev: optional device uint64 added to `offset` on the device (the per-step counter of a replayed step plan)."""
     _ck(lib.semseg_dropout2d_mask(_p(mask), mask.numel(), float(p), int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset),
