@@ -303,16 +303,18 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
  * class; row (i, j)'s alternative a is element i * tn + j * tp + a * tk of top_ids / top_logprobs.  Any output may be NULL.  stats
  * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
  * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
+ * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes), nothing needs to be cleared.
  * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (the ids stay in range, NaN first).
  * semseg_class_logprobs_bwd: dz (=|+=) the gradient from those of logprob, entropy, lse (each may be NULL); 0 for rows that are void
  * or hold only -inf; strides dn, dp, dc; dz has the logits' type, one rounding. */
 enum { SEMSEG_TYPE_F32 = 0, SEMSEG_TYPE_BF16 = 1, SEMSEG_TYPE_F16 = 2 };
 enum { SEMSEG_REDUCE_NONE = 0, SEMSEG_REDUCE_MEAN = 1, SEMSEG_REDUCE_SUM = 2 };
 enum { SEMSEG_CLASS_TOP_MAX = 64 };
+size_t semseg_class_logprobs_scratch_bytes(int type, long long n, long long p, int C, long long sc, int k);
 int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
                               long long sc, const long long* label, long long ignore_index, float T, int k, float* logprob,
                               float* entropy, float* lse, float* stats, int* top_ids, float* top_logprobs, long long tn,
-                              long long tp, long long tk, hipStream_t stream);
+                              long long tp, long long tk, void* scratch, size_t scratch_bytes, hipStream_t stream);
 int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
                               long long sc, const long long* label, long long ignore_index, float T, const float* stats,
                               const float* entropy, const float* g_logprob, const float* g_entropy, const float* g_lse,

@@ -28,7 +28,7 @@ __device__ __forceinline__ void store1(_Float16* p, float v) { *p = (_Float16)v;
 __device__ __forceinline__ unsigned order_key(float z) {
   const unsigned u = __float_as_uint(z + 0.f);
   const unsigned k = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
-  return z != z ? 0xffffffffu : k;
+  return z != z ? 0xfffffffeu : k;
 }
 // ... with the class as the second criterion: the lowest one first
 __device__ __forceinline__ unsigned long long pair_key(float z, int c) {
@@ -52,12 +52,100 @@ __device__ __forceinline__ unsigned long long wave_max64(unsigned long long v) {
   return v;
 }
 
+// ---- reductions over groups of G = 8 or 64 neighbouring lanes: data-parallel moves inside a row of 16, a shuffle across rows
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
+template <int G, typename T, typename F>
+__device__ __forceinline__ T group_reduce(T v, F f) {
+  v = f(v, dpp<XOR1>(v));
+  v = f(v, dpp<XOR2>(v));
+  v = f(v, dpp<HALF_MIRROR>(v));
+  if (G == 64) {
+    v = f(v, dpp<MIRROR>(v));
+    v = f(v, __shfl_xor(v, 16));
+    v = f(v, __shfl_xor(v, 32));
+  }
+  return v;
+}
+template <int G> __device__ __forceinline__ float group_max(float v) { return group_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int G> __device__ __forceinline__ float group_sum(float v) { return group_reduce<G>(v, [](float a, float b) { return a + b; }); }
+template <int G> __device__ __forceinline__ unsigned group_umax(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a > b ? a : b; }); }
+template <int G> __device__ __forceinline__ unsigned group_umin(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a < b ? a : b; }); }
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }
+
+// ---- 16 bytes of logits at an element's own alignment: rows of odd lengths start anywhere, and global loads and stores of this hardware
+// need no more than that
+template <typename E> constexpr int VEC = 16 / (int)sizeof(E);
+template <typename E>
+using Vec = E __attribute__((ext_vector_type(16 / sizeof(E))));
+template <typename E>
+struct __attribute__((packed, aligned(alignof(E)))) Raw { u32x4 v; };
+template <typename E>
+__device__ __forceinline__ void load_vec(const E* p, float (&x)[VEC<E>]) {
+  const Vec<E> q = __builtin_bit_cast(Vec<E>, reinterpret_cast<const Raw<E>*>(p)->v);
+#pragma unroll
+  for (int e = 0; e < VEC<E>; ++e) x[e] = (float)q[e];
+}
+template <typename E>
+__device__ __forceinline__ void store_vec(E* p, const float (&x)[VEC<E>]) {
+  Vec<E> q;
+#pragma unroll
+  for (int e = 0; e < VEC<E>; ++e) q[e] = (E)x[e];
+  reinterpret_cast<Raw<E>*>(p)->v = __builtin_bit_cast(u32x4, q);
+}
+// VEC classes of a row of C from class s on; what lies beyond the row is -inf and not read.  Returns the class of x[0]: the row's last
+// chunk is loaded from C - VEC, its classes below s (another lane has them) made -inf too.  SHORT: C may be less than VEC.
+template <bool SHORT = false, typename E>
+__device__ __forceinline__ int load_chunk(const E* z, int s, int C, float (&x)[VEC<E>]) {
+  constexpr int V = VEC<E>;
+  if (!SHORT || C >= V) {
+    const int b = min(s, C - V);
+    load_vec(z + b, x);
+    if (b != s) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = b + e >= s ? x[e] : -INFINITY;
+    }
+    return b;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) x[e] = s + e < C ? load1(z + s + e) : -INFINITY;
+  return s;
+}
+template <typename E>
+__device__ __forceinline__ void store_chunk(E* z, int s, int b, int C, const float (&x)[VEC<E>]) {
+  if (s + VEC<E> <= C) {
+    store_vec(z + s, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC<E>; ++e)
+      if (b + e >= s && b + e < C) store1(z + b + e, x[e]);
+  }
+}
+
+// i * s0 + j * s1 of row r = i * p + j; 64-bit divisions (~150 instructions) are kept out of the usual cases
+__device__ __forceinline__ long long row_at(long long r, long long p, long long R, long long s0, long long s1) {
+  if (p == R) return r * s1;
+  if (R <= 0x7fffffff) {
+    const unsigned i = (unsigned)r / (unsigned)p;
+    return i * s0 + ((unsigned)r - i * (unsigned)p) * s1;
+  }
+  return (r / p) * s0 + (r % p) * s1;
+}
+
 struct Logits {
   const void* z;
   long long R, p, sn, sp, sc;
   int C;
   float invT, scale2;      // 1 / T, log2(e) / T
-  __device__ __forceinline__ long long at(long long r) const { return (r / p) * sn + (r % p) * sp; }
+  __device__ __forceinline__ long long at(long long r) const { return row_at(r, p, R, sn, sp); }
 };
 
 struct LogprobOut {
@@ -70,6 +158,30 @@ struct LogprobOut {
   long long tn, tp, tk;
 };
 
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// s, u taken about `from` become sums about `to` >= from (u's terms carry a factor d); an empty sum may come from -inf
+__device__ __forceinline__ void rescale(float& s, float& u, float from, float to, float scale2) {
+  const float d = (from - to) * scale2, f = exp2_(d);
+  u = (u + s * fmaxf(d, -300.f)) * f;
+  s = s * f;
+}
+
+__device__ __forceinline__ void void_row(const LogprobOut& o, long long r, long long R) {
+  if (o.logprob) o.logprob[r] = 0.f;
+  if (o.entropy) o.entropy[r] = 0.f;
+  if (o.lse) o.lse[r] = 0.f;
+  if (o.stats) o.stats[r] = o.stats[R + r] = 0.f;
+}
+// s = sum exp2(d), u = sum exp2(d) d about base, ls = log s; s = 0: every logit is -inf
+__device__ __forceinline__ void finish_row(const LogprobOut& o, long long r, const Logits& a, float base, float s, float u, float ls,
+                                           bool is_class, float zy) {
+  if (o.stats) { o.stats[r] = base; o.stats[a.R + r] = ls; }
+  if (o.lse) o.lse[r] = base * a.invT + ls;
+  if (o.entropy) o.entropy[r] = s == 0.f ? 0.f : ls - u / s * LN2;
+  if (o.logprob) o.logprob[r] = !is_class ? NAN : s == 0.f ? -INFINITY : (zy - base) * a.invT - ls;
+}
+
 // One wave per row, lanes along the classes: any strides.
 template <typename E>
 __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const LogprobOut o) {
@@ -78,14 +190,9 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += waves) {
     const E* z = (const E*)a.z + a.at(r);
     const long long y = o.label ? o.label[r] : 0;
-    const long long ot = (r / a.p) * o.tn + (r % a.p) * o.tp;
+    const long long ot = row_at(r, a.p, a.R, o.tn, o.tp);
     if (o.label && y == o.ignore) {            // a void row is not read
-      if (lane == 0) {
-        if (o.logprob) o.logprob[r] = 0.f;
-        if (o.entropy) o.entropy[r] = 0.f;
-        if (o.lse) o.lse[r] = 0.f;
-        if (o.stats) o.stats[r] = o.stats[a.R + r] = 0.f;
-      }
+      if (lane == 0) void_row(o, r, a.R);
       if (lane < o.k) {
         o.top_ids[ot + lane * o.tk] = -1;
         o.top_lp[ot + lane * o.tk] = -INFINITY;
@@ -98,21 +205,15 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
     const float base = m == -INFINITY ? 0.f : m;
     float s = 0.f, u = 0.f;
     for (int c = lane; c < a.C; c += 64) {
-      const float d = (load1(z + c * a.sc) - base) * a.scale2, e = exp2f(d);
+      const float d = (load1(z + c * a.sc) - base) * a.scale2, e = exp2_(d);
       s += e;
       u += e * fmaxf(d, -300.f);               // exp2(-300) = 0 in fp32; 0 * -inf would be NaN
     }
     s = wave_sum(s);
     u = wave_sum(u);
-    const bool none = s == 0.f;                // every logit -inf
-    const float ls = logf(s);
-    if (lane == 0) {
-      if (o.stats) { o.stats[r] = base; o.stats[a.R + r] = ls; }
-      if (o.lse) o.lse[r] = base * a.invT + ls;
-      if (o.entropy) o.entropy[r] = none ? 0.f : ls - u / s * LN2;
-      if (o.logprob)
-        o.logprob[r] = (y < 0 || y >= a.C) ? NAN : none ? -INFINITY : (load1(z + y * a.sc) - base) * a.invT - ls;
-    }
+    const float ls = log2_(s) * LN2;
+    const bool is_class = y >= 0 && y < a.C;
+    if (lane == 0) finish_row(o, r, a, base, s, u, ls, is_class, o.logprob && is_class ? load1(z + y * a.sc) : 0.f);
     unsigned long long prev = ~0ull;
     for (int j = 0; j < o.k; ++j) {
       unsigned long long best = 0;
@@ -124,8 +225,346 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
       if (lane == 0) {
         const int c = (int)~(unsigned)prev;
         o.top_ids[ot + j * o.tk] = c;
-        o.top_lp[ot + j * o.tk] = none ? -INFINITY : (load1(z + c * a.sc) - base) * a.invT - ls;
+        o.top_lp[ot + j * o.tk] = s == 0.f ? -INFINITY : (load1(z + c * a.sc) - base) * a.invT - ls;
       }
+    }
+  }
+}
+
+// Rows of at most 2048 contiguous classes: G lanes (8 up to 256 classes, 64 beyond) hold a row in registers, NV chunks of 16 bytes each,
+// so it is read once and its maximum, sums and alternatives are reductions over registers and a few data-parallel moves.
+// An alternative is one round over the G lanes' order keys: the largest key, the lowest class that has it, that class taken out.
+template <typename E, int G, int NV>
+__global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, const LogprobOut o) {
+  constexpr int V = VEC<E>;
+  const int l = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * (256 / G);
+  for (long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; r < a.R; r += step) {
+    const long long y = o.label ? o.label[r] : 0;
+    const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+    if (o.label && y == o.ignore) {
+      if (l == 0) void_row(o, r, a.R);
+      for (int j = l; j < o.k; j += G) {
+        o.top_ids[ot + j * o.tk] = -1;
+        o.top_lp[ot + j * o.tk] = -INFINITY;
+      }
+      continue;
+    }
+    const E* z = (const E*)a.z + a.at(r);
+    float x[NV][V];
+    int b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) b[i] = load_chunk<G == 8 && NV == 1>(z, (i * G + l) * V, a.C, x[i]);
+    float zy = 0.f;
+    const bool is_class = y >= 0 && y < a.C;
+    if (l == 0 && o.logprob && is_class) zy = load1(z + y);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, x[i][e]);
+    m = group_max<G>(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = (x[i][e] - base) * a.scale2, w = exp2_(d);
+        s += w;
+        u += w * fmaxf(d, -300.f);               // exp2(-300) = 0 in fp32; 0 * -inf would be NaN
+      }
+    s = group_sum<G>(s);
+    u = group_sum<G>(u);
+    const float ls = log2_(s) * LN2;
+    if (l == 0) finish_row(o, r, a, base, s, u, ls, is_class, zy);
+    if (o.k == 0) continue;
+    unsigned key[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const int c = b[i] + e;
+        key[i][e] = c >= (i * G + l) * V && c < a.C ? order_key(x[i][e]) : 0u;
+      }
+    for (int j = 0; j < o.k; ++j) {
+      unsigned best = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) best = max(best, key[i][e]);
+      best = group_umax<G>(best);
+      unsigned c = 0xffffffffu;
+#pragma unroll
+      for (int i = NV - 1; i >= 0; --i)
+#pragma unroll
+        for (int e = V - 1; e >= 0; --e) c = key[i][e] == best ? (unsigned)(b[i] + e) : c;
+      c = group_umin<G>(c);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) key[i][e] = (unsigned)(b[i] + e) == c ? 0u : key[i][e];
+      if (l == (j & (G - 1))) {
+        o.top_ids[ot + j * o.tk] = (int)c;
+        o.top_lp[ot + j * o.tk] = s == 0.f ? -INFINITY : (key_value(best) - base) * a.invT - ls;
+      }
+    }
+  }
+}
+
+// Rows of more classes: a block of 256 lanes streams a slice of a row (the whole row where there are rows enough), 16 bytes a lane and
+// load, and keeps each lane's running maximum and sums, rescaled once per four loads.  The k best come out of the same pass: the 8 lanes
+// that read one 128-byte line note its maximum in LDS (for rows beyond 4096 lines, that of `join` lines of theirs).  Afterwards
+//   tau = the k-th largest of the 256 lanes' maxima over their lines' maxima (a bound: at least k logits are >= tau),
+//   the lines whose maximum is >= tau are read again (about k of them), their logits >= tau collected and ranked by counting.
+// With many equal logits the lists could run over: then (and where a NaN hides from the maxima) the k best are taken in k passes.
+constexpr int LINES = 4096, CAND = 512, CLINES = 256;
+
+struct Stream {
+  long long r0;                       // first row of this launch
+  int nsplit, slice, join;            // slices of a row, classes of one (a multiple of VEC), lines whose maximum is kept together
+  float* part;                        // [R][nsplit][3]: maximum, sum, sum of e d (nsplit > 1)
+  unsigned long long* keys;           // [R][nsplit][k] (nsplit > 1)
+};
+
+template <typename E>
+__global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, const LogprobOut o, const Stream t) {
+  constexpr int V = VEC<E>;
+  __shared__ unsigned line[LINES];
+  __shared__ unsigned long long cand[CAND];
+  __shared__ int clist[CLINES];
+  __shared__ float red[3][4];
+  __shared__ unsigned long long red64[4];
+  __shared__ unsigned tau_s;
+  __shared__ int nlines, ncand;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, g8 = tid >> 3;
+  const int sp = (int)(blockIdx.x % (unsigned)t.nsplit);
+  const long long r = t.r0 + blockIdx.x / (unsigned)t.nsplit;
+  const long long y = o.label ? o.label[r] : 0;
+  const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+  if (o.label && y == o.ignore) {      // with several slices the joining kernel writes the row
+    if (t.nsplit == 1) {
+      if (tid == 0) void_row(o, r, a.R);
+      if (tid < o.k) {
+        o.top_ids[ot + tid * o.tk] = -1;
+        o.top_lp[ot + tid * o.tk] = -INFINITY;
+      }
+    }
+    return;
+  }
+  const E* z = (const E*)a.z + a.at(r);
+  const int c0 = sp * t.slice, c1 = min(a.C, c0 + t.slice);
+  const int iters = (c1 - c0 + 256 * V - 1) / (256 * V);
+  float m = -INFINITY, s = 0.f, u = 0.f, lm = -INFINITY;
+  constexpr int UN = 4;
+  for (int it = 0; it < iters; it += UN) {
+    float x[UN][V], cm[UN];
+    if (c0 + (it + UN) * 256 * V <= c1) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n) load_vec(z + c0 + ((it + n) * 256 + tid) * V, x[n]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const int c = c0 + ((it + n) * 256 + tid) * V;
+        if (c < c1) {
+          load_chunk(z, c, a.C, x[n]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[n][e] = -INFINITY;
+        }
+      }
+    }
+    float nm = m;
+#pragma unroll
+    for (int n = 0; n < UN; ++n) {
+      cm[n] = x[n][0];
+#pragma unroll
+      for (int e = 1; e < V; ++e) cm[n] = fmaxf(cm[n], x[n][e]);
+      nm = fmaxf(nm, cm[n]);
+    }
+    if (o.k) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        lm = fmaxf(lm, group_max<8>(cm[n]));
+        const int q = it + n;
+        if (q < iters && ((q + 1) % t.join == 0 || q + 1 == iters)) {
+          if ((tid & 7) == 0) line[(q / t.join) * 32 + g8] = order_key(lm);
+          lm = -INFINITY;
+        }
+      }
+    }
+    const float base = nm == -INFINITY ? 0.f : nm;
+    rescale(s, u, m, base, a.scale2);
+    m = nm;
+#pragma unroll
+    for (int n = 0; n < UN; ++n)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = (x[n][e] - base) * a.scale2, w = exp2_(d);
+        s += w;
+        u += w * fmaxf(d, -300.f);
+      }
+  }
+  // join the lanes, then the waves
+  const float wm = group_max<64>(m);
+  rescale(s, u, m, wm == -INFINITY ? 0.f : wm, a.scale2);
+  s = group_sum<64>(s);
+  u = group_sum<64>(u);
+  if (lane == 0) { red[0][wv] = wm; red[1][wv] = s; red[2][wv] = u; }
+  if (tid == 0) nlines = ncand = 0;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  const float base = m == -INFINITY ? 0.f : m;
+  s = u = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    float sw = red[1][w], uw = red[2][w];
+    rescale(sw, uw, red[0][w], base, a.scale2);
+    s += sw;
+    u += uw;
+  }
+  const float ls = log2_(s) * LN2;
+  if (tid == 0) {
+    if (t.nsplit > 1) {
+      float* q = t.part + (r * t.nsplit + sp) * 3;
+      q[0] = m;
+      q[1] = s;
+      q[2] = u;
+    } else {
+      const bool is_class = y >= 0 && y < a.C;
+      finish_row(o, r, a, base, s, u, ls, is_class, o.logprob && is_class ? load1(z + y) : 0.f);
+    }
+  }
+  if (o.k == 0) return;
+
+  const int nl = ((iters + t.join - 1) / t.join) * 32;
+  unsigned best = 0;
+  for (int i = tid; i < nl; i += 256) best = max(best, line[i]);
+  cand[tid] = best;
+  __syncthreads();
+  if (wv == 0) {                       // the k-th largest of the 256 maxima, bit by bit
+    unsigned q[4], tau = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = (unsigned)cand[i * 64 + lane];
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned c = tau | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n += __popcll(__ballot(q[i] >= c));
+      if (n >= o.k) tau = c;
+    }
+    if (lane == 0) tau_s = tau > 1u ? tau : 1u;
+  }
+  __syncthreads();
+  const unsigned tau = tau_s;
+  for (int i = tid; i < nl; i += 256)
+    if (line[i] >= tau) {
+      const int n = atomicAdd(&nlines, 1);
+      if (n < CLINES) clist[n] = i;
+    }
+  __syncthreads();
+  bool slow = nlines > CLINES || !(s < INFINITY);
+  if (!slow) {
+    for (int i = g8; i < nlines; i += 32) {
+      const int li = clist[i];
+      for (int j = 0; j < t.join; ++j) {
+        const int c = c0 + (((li / 32) * t.join + j) * 256 + (li % 32) * 8 + (tid & 7)) * V;
+        if (c >= c1) continue;
+        float x[V];
+        const int b = load_chunk(z, c, a.C, x);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (b + e >= c && b + e < a.C && order_key(x[e]) >= tau) {
+            const int n = atomicAdd(&ncand, 1);
+            if (n < CAND) cand[n] = pair_key(x[e], b + e);
+          }
+      }
+    }
+  }
+  __syncthreads();
+  slow = slow || ncand > CAND;
+  int n = ncand;
+  if (slow) {
+    unsigned long long prev = ~0ull;
+    n = 0;
+    for (int j = 0; j < o.k; ++j) {
+      unsigned long long top = 0;
+      for (int c = c0 + tid; c < c1; c += 256) {
+        const unsigned long long key = pair_key(load1(z + c), c);
+        if (key < prev && key > top) top = key;
+      }
+      top = wave_max64(top);
+      __syncthreads();
+      if (lane == 0) red64[wv] = top;
+      __syncthreads();
+      for (int w = 0; w < 4; ++w) top = red64[w] > top ? red64[w] : top;
+      prev = top;
+      if (top) n = j + 1;
+      if (tid == 0) cand[j] = top;
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < n; i += 256) {
+    const unsigned long long key = cand[i];
+    int rank = i;
+    if (!slow) {
+      rank = 0;
+      for (int j = 0; j < n; ++j) rank += cand[j] > key;
+    }
+    if (rank < o.k) {
+      if (t.nsplit > 1) {
+        t.keys[(r * t.nsplit + sp) * o.k + rank] = key;
+      } else {
+        o.top_ids[ot + rank * o.tk] = (int)~(unsigned)key;
+        o.top_lp[ot + rank * o.tk] = s == 0.f ? -INFINITY : (key_value((unsigned)(key >> 32)) - base) * a.invT - ls;
+      }
+    }
+  }
+  if (t.nsplit > 1)                    // a short last slice
+    for (int i = n + tid; i < o.k; i += 256) t.keys[(r * t.nsplit + sp) * o.k + i] = 0;
+}
+
+// One wave joins the slices of a row, a lane to a slice: sums by the joint maximum, alternatives by merging the slices' falling lists.
+template <typename E>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(const Logits a, const LogprobOut o, const Stream t) {
+  const int lane = threadIdx.x;
+  const long long r = t.r0 + blockIdx.x;
+  const long long y = o.label ? o.label[r] : 0;
+  const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+  if (o.label && y == o.ignore) {
+    if (lane == 0) void_row(o, r, a.R);
+    if (lane < o.k) {
+      o.top_ids[ot + lane * o.tk] = -1;
+      o.top_lp[ot + lane * o.tk] = -INFINITY;
+    }
+    return;
+  }
+  const bool on = lane < t.nsplit;
+  const float* q = t.part + (r * t.nsplit + (on ? lane : 0)) * 3;
+  const float m1 = on ? q[0] : -INFINITY;
+  float s = on ? q[1] : 0.f, u = on ? q[2] : 0.f;
+  const unsigned long long* keys = t.keys + (r * t.nsplit + (on ? lane : 0)) * o.k;
+  unsigned long long head = on && o.k ? keys[0] : 0;
+  const float m = group_max<64>(m1);
+  const float base = m == -INFINITY ? 0.f : m;
+  rescale(s, u, m1, base, a.scale2);
+  s = group_sum<64>(s);
+  u = group_sum<64>(u);
+  const float ls = log2_(s) * LN2;
+  if (lane == 0) {
+    const bool is_class = y >= 0 && y < a.C;
+    finish_row(o, r, a, base, s, u, ls, is_class, o.logprob && is_class ? load1((const E*)a.z + a.at(r) + y) : 0.f);
+  }
+  int at = 0;
+  for (int j = 0; j < o.k; ++j) {
+    const unsigned long long top = wave_max64(head);
+    if (head == top) {
+      ++at;
+      head = on && at < o.k ? keys[at] : 0;
+    }
+    if (lane == 0) {
+      o.top_ids[ot + j * o.tk] = (int)~(unsigned)top;
+      o.top_lp[ot + j * o.tk] = s == 0.f ? -INFINITY : (key_value((unsigned)(top >> 32)) - base) * a.invT - ls;
     }
   }
 }
@@ -146,7 +585,7 @@ __global__ __launch_bounds__(256) void logprobs_bwd_kernel(const Logits a, const
   const long long waves = (long long)gridDim.x * 4;
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += waves) {
     const E* z = (const E*)a.z + a.at(r);
-    E* dz = (E*)g.dz + (r / a.p) * g.dn + (r % a.p) * g.dp;
+    E* dz = (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp);
     const long long y = g.label ? g.label[r] : -1;
     const float m = g.stats[r], ls = g.stats[a.R + r];
     if ((g.label && y == g.ignore) || ls == -INFINITY) {
@@ -174,12 +613,13 @@ struct Teacher {
   int ids64, top_type, k, tail;
   long long in, ip, ik, vn, vp, vk;
   const float* weight;
-  __device__ __forceinline__ long long id(long long r, long long p, int j) const {
-    const long long o = (r / p) * in + (r % p) * ip + j * ik;
+  // entry j of the row whose entries start at io / vo
+  __device__ __forceinline__ long long id(long long io, int j) const {
+    const long long o = io + j * ik;
     return ids64 ? ((const long long*)ids)[o] : ((const int*)ids)[o];
   }
-  __device__ __forceinline__ float value(long long r, long long p, int j) const {
-    const long long o = (r / p) * vn + (r % p) * vp + j * vk;
+  __device__ __forceinline__ float value(long long vo, int j) const {
+    const long long o = vo + j * vk;
     return top_type == SEMSEG_TYPE_F32 ? ((const float*)top)[o]
          : top_type == SEMSEG_TYPE_BF16 ? (float)((const __bf16*)top)[o] : (float)((const _Float16*)top)[o];
   }
@@ -187,16 +627,16 @@ struct Teacher {
 
 // The teacher's distribution of one row, entry j in lane j (k <= 64): q, log q; qsum = sum q, qrest = what is left of 1 (tail).
 // id -1 where the entry is absent (negative id, lane >= k); *bad: an id >= C.
-__device__ __forceinline__ void teacher_row(const Teacher& t, long long r, long long p, int C, float invT, int lane, int& id, float& q,
+__device__ __forceinline__ void teacher_row(const Teacher& t, long long r, const Logits& a, int lane, int& id, float& q,
                                             float& lq, float& qsum, float& qrest, bool& bad) {
   long long i = -1;
   float v = -INFINITY;
   if (lane < t.k) {
-    i = t.id(r, p, lane);
-    if (i >= 0) v = t.value(r, p, lane);
+    i = t.id(row_at(r, a.p, a.R, t.in, t.ip), lane);
+    if (i >= 0) v = t.value(row_at(r, a.p, a.R, t.vn, t.vp), lane);
   }
-  bad = __any(i >= C);
-  id = i < 0 || i >= C ? -1 : (int)i;
+  bad = __any(i >= a.C);
+  id = i < 0 || i >= a.C ? -1 : (int)i;
   if (id < 0) v = -INFINITY;
   if (t.tail) {
     lq = v;
@@ -205,7 +645,7 @@ __device__ __forceinline__ void teacher_row(const Teacher& t, long long r, long 
     qrest = fmaxf(1.f - qsum, 0.f);
   } else {
     const float m = wave_max(v);
-    const float d = (v - (m == -INFINITY ? 0.f : m)) * invT;
+    const float d = (v - (m == -INFINITY ? 0.f : m)) * a.invT;
     const float e = expf(d), s = wave_sum(e);
     lq = d - logf(s);
     q = s == 0.f ? 0.f : e / s;
@@ -238,7 +678,7 @@ __global__ __launch_bounds__(256) void distill_fwd_kernel(const Logits a, const 
     int id;
     float q, lq, qsum, qrest;
     bool bad;
-    teacher_row(t, r, a.p, a.C, a.invT, lane, id, q, lq, qsum, qrest, bad);
+    teacher_row(t, r, a, lane, id, q, lq, qsum, qrest, bad);
     float m = -INFINITY, mt = -INFINITY;
     for (int c0 = 0; c0 < a.C; c0 += 64) {
       const int c = c0 + lane;
@@ -329,13 +769,13 @@ __global__ __launch_bounds__(256) void distill_bwd_kernel(const Logits a, const 
   const long long waves = (long long)gridDim.x * 4;
   for (long long r = (long long)blockIdx.x * 4 + wv; r < a.R; r += waves) {
     const E* z = (const E*)a.z + a.at(r);
-    E* dz = (E*)g.dz + (r / a.p) * g.dn + (r % a.p) * g.dp;
+    E* dz = (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp);
     const float w = t.weight ? t.weight[r] : 1.f;
     const float base = g.stats[r], ls = g.stats[a.R + r], lpt = g.stats[2 * a.R + r];
     int id;
     float q, lq, qsum, qrest;
     bool bad;
-    teacher_row(t, r, a.p, a.C, a.invT, lane, id, q, lq, qsum, qrest, bad);
+    teacher_row(t, r, a, lane, id, q, lq, qsum, qrest, bad);
     float coef = g.gmul * g.T * w * (g.g ? g.g[g.per_row ? r : 0] : 1.f);
     if (g.mean) coef = g.acc[1] == 0.0 ? 0.f : (float)((double)coef / g.acc[1]);
     if (w == 0.f || bad || ls == -INFINITY || !__any(id >= 0)) {
@@ -380,6 +820,57 @@ Logits logits_of(const void* z, long long n, long long p, int C, long long sn, l
   return Logits{z, n * p, p, sn, sp, sc, C, 1.f / T, LOG2E / T};
 }
 
+// Slices of a row of more classes than ROW_CLASSES: none with 512 rows or more (two blocks a compute unit), else about 1024 blocks in
+// all, a slice no shorter than 4096 classes.
+constexpr int ROW_CLASSES = 2048;
+struct Split { int nsplit, slice, join; };
+Split split_rows(int type, long long R, int C) {
+  const int v = type == SEMSEG_TYPE_F32 ? 4 : 8;
+  if (C <= ROW_CLASSES) return Split{1, C, 1};
+  long long n = R >= 512 ? 1 : 1024 / R;
+  if (n > 64) n = 64;
+  if (n > (C + 4095) / 4096) n = (C + 4095) / 4096;
+  const int slice = (int)(((C + n - 1) / n + v - 1) / v * v);
+  const int iters = (slice + 256 * v - 1) / (256 * v);
+  return Split{(C + slice - 1) / slice, slice, (iters + 127) / 128};
+}
+int capped(long long blocks, int cap) { return (int)(blocks < cap ? blocks : cap); }
+
+template <typename E>
+void logprobs_fwd(const Logits& a, const LogprobOut& o, int type, void* scratch, hipStream_t stream) {
+  if (a.C > 1 && a.sc != 1) {
+    logprobs_fwd_kernel<E><<<row_blocks(a.R), 256, 0, stream>>>(a, o);
+    return;
+  }
+  if (a.C <= ROW_CLASSES) {
+    const int chunks = (a.C + VEC<E> - 1) / VEC<E>;
+#define ROWS(G, NV) logprobs_rows_kernel<E, G, NV><<<capped((a.R + 256 / G - 1) / (256 / G), 16384), 256, 0, stream>>>(a, o)
+    if (chunks <= 8) ROWS(8, 1);
+    else if (chunks <= 16) ROWS(8, 2);
+    else if (chunks <= 24) ROWS(8, 3);
+    else if (chunks <= 32) ROWS(8, 4);
+    else if (VEC<E> == 4 && chunks <= 40) ROWS(8, VEC<E> == 4 ? 5 : 1);
+    else if (VEC<E> == 4 && chunks <= 64) ROWS(8, VEC<E> == 4 ? 8 : 1);
+    else if (chunks <= 64) ROWS(64, 1);
+    else if (chunks <= 128) ROWS(64, 2);
+    else if (chunks <= 256) ROWS(64, 4);
+    else ROWS(64, VEC<E> == 4 ? 8 : 1);
+#undef ROWS
+    return;
+  }
+  const Split s = split_rows(type, a.R, a.C);
+  Stream t{0, s.nsplit, s.slice, s.join, (float*)scratch, nullptr};
+  // the keys first in the scratch: they need 8-byte alignment
+  t.keys = (unsigned long long*)scratch;
+  t.part = (float*)(t.keys + a.R * s.nsplit * o.k);
+  const long long most = (1ll << 23) / s.nsplit;       // a grid holds less than 2^32 lanes
+  for (t.r0 = 0; t.r0 < a.R; t.r0 += most) {
+    const int rows = (int)(a.R - t.r0 < most ? a.R - t.r0 : most);
+    logprobs_stream_kernel<E><<<rows * s.nsplit, 256, 0, stream>>>(a, o, t);
+    if (s.nsplit > 1) logprobs_join_kernel<E><<<rows, 64, 0, stream>>>(a, o, t);
+  }
+}
+
 #define BY_TYPE(type, K, ...)                            \
   do {                                                   \
     if (type == SEMSEG_TYPE_F32) K<float> __VA_ARGS__;   \
@@ -391,15 +882,25 @@ Logits logits_of(const void* z, long long n, long long p, int C, long long sn, l
 
 extern "C" {
 
+size_t semseg_class_logprobs_scratch_bytes(int type, long long n, long long p, int C, long long sc, int k) {
+  if (n <= 0 || p <= 0 || C <= 0 || k < 0 || (sc != 1 && C > 1)) return 0;
+  const Split s = split_rows(type, n * p, C);
+  return s.nsplit < 2 ? 0 : (size_t)(n * p) * s.nsplit * (3 * sizeof(float) + k * sizeof(unsigned long long));
+}
+
 int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp, long long sc,
                               const long long* label, long long ignore_index, float T, int k, float* logprob, float* entropy,
                               float* lse, float* stats, int* top_ids, float* top_logprobs, long long tn, long long tp, long long tk,
-                              hipStream_t stream) {
+                              void* scratch, size_t scratch_bytes, hipStream_t stream) {
   if (!logits_ok(z, type, n, p, C, T) || k < 0 || k > MAXK || k > C || (k && (!top_ids || !top_logprobs)) || (logprob && !label))
     return SEMSEG_EINVAL;
+  const size_t need = semseg_class_logprobs_scratch_bytes(type, n, p, C, sc, k);
+  if (need && (!scratch || scratch_bytes < need)) return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
   const LogprobOut o{label, ignore_index, logprob, entropy, lse, stats, top_ids, top_logprobs, k, tn, tp, tk};
-  BY_TYPE(type, logprobs_fwd_kernel, <<<row_blocks(a.R), 256, 0, stream>>>(a, o));
+  if (type == SEMSEG_TYPE_F32) logprobs_fwd<float>(a, o, type, scratch, stream);
+  else if (type == SEMSEG_TYPE_BF16) logprobs_fwd<__bf16>(a, o, type, scratch, stream);
+  else logprobs_fwd<_Float16>(a, o, type, scratch, stream);
   return semseg_launch_status();
 }
 

@@ -135,7 +135,10 @@ class _Logprobs(torch.autograd.Function):
             if k:
                 ids, tlp = g.empty(k, torch.int32, z.device), g.empty(k, torch.float32, z.device)
                 ts = g.strides_of(ids)
-            ops.class_logprobs_fwd(z, g.geom, g.strides, label, ignore_index, temperature, k, logprob, entropy, lse, stats, ids, tlp, ts)
+            need = ops.class_logprobs_scratch_bytes(z.dtype, *g.geom, g.strides[2], k)
+            scratch = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
+            ops.class_logprobs_fwd(z, g.geom, g.strides, label, ignore_index, temperature, k, logprob, entropy, lse, stats, ids, tlp, ts,
+                                   scratch)
         ctx.save_for_backward(z, label, stats, entropy)
         ctx.g, ctx.ignore_index, ctx.temperature = g, ignore_index, temperature
         ctx.mark_non_differentiable(*[t for t in (ids, tlp) if t is not None])

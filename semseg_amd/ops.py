@@ -576,11 +576,15 @@ REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def class_logprobs_fwd(z, geom, strides, label, ignore_index, T, k, logprob, entropy, lse, stats, top_ids=None, top_logprobs=None,
-                       top_strides=(0, 0, 0)):
+                       top_strides=(0, 0, 0), scratch=None):
     """geom (n, p, C), strides (sn, sp, sc): rows i * p + j of z (include/semseg_hip.h); logits of an fp32 / bf16 / fp16 tensor."""
     _ck(lib.semseg_class_logprobs_fwd(_p(z), TYPES[z.dtype], *geom, *strides, _p(label), int(ignore_index), float(T), k,
                                       _p(logprob), _p(entropy), _p(lse), _p(stats), _p(top_ids), _p(top_logprobs), *top_strides,
-                                      _stream()), "class_logprobs_fwd")
+                                      _p(scratch), 0 if scratch is None else scratch.numel(), _stream()), "class_logprobs_fwd")
+
+
+def class_logprobs_scratch_bytes(dtype, n, p, C, sc, k):
+    return int(lib.semseg_class_logprobs_scratch_bytes(TYPES[dtype], n, p, C, sc, k))
 
 
 def class_logprobs_bwd(z, geom, strides, label, ignore_index, T, stats, entropy, g_logprob, g_entropy, g_lse, dz, dstrides,

@@ -85,10 +85,12 @@ def test_the_c_entries_refuse_bad_arguments_without_a_gpu():
     p = 4096      # never read: every call below is refused on the host
     none3, s3 = (0, 0, 0), (0, 8, 1)
     fwd = lambda z=p, t=0, n=1, pp=4, C=8, T=1.0, k=0, lp=None, ids=None, lab=None: lib.semseg_class_logprobs_fwd(  # noqa: E731
-        z, t, n, pp, C, *s3, lab, 255, T, k, lp, None, None, None, ids, ids, *none3, None)
+        z, t, n, pp, C, *s3, lab, 255, T, k, lp, None, None, None, ids, ids, *none3, None, 0, None)
     for kw in (dict(z=None), dict(t=3), dict(t=-1), dict(n=0), dict(pp=0), dict(C=0), dict(T=0.0), dict(T=-1.0), dict(T=math.nan),
                dict(T=math.inf), dict(k=-1), dict(k=1), dict(k=9, ids=p), dict(C=100, k=65, ids=p), dict(lp=p), dict(n=1 << 30, pp=1 << 30)):
         assert fwd(**kw) == -1, kw
+    assert fwd(C=100000) == -1                  # one row in several slices needs scratch
+    assert lib.semseg_class_logprobs_scratch_bytes(0, 1, 4, 8, 1, 5) == 0 < lib.semseg_class_logprobs_scratch_bytes(0, 1, 1, 100000, 1, 5)
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, None, None, None, None, None, p, *s3, 0, None) == -1
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, p, None, p, None, None, p, *s3, 0, None) == -1
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, p, None, None, p, None, p, *s3, 0, None) == -1
