@@ -569,6 +569,215 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const Logits a, const
   }
 }
 
+// ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane
+template <typename E, int PV>
+__device__ __forceinline__ void load_px(const E* p, E (&q)[PV]) {
+  if constexpr (PV * sizeof(E) == 4) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
+    const unsigned w = reinterpret_cast<const W*>(p)->v;
+    __builtin_memcpy(q, &w, 4);
+  } else if constexpr (PV * sizeof(E) == 8) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
+    const u32x2 w = reinterpret_cast<const W*>(p)->v;
+    __builtin_memcpy(q, &w, 8);
+  } else {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) q[v] = p[v];
+  }
+}
+template <typename E, int PV>
+__device__ __forceinline__ void store_px(E* p, const E (&q)[PV]) {
+  if constexpr (PV * sizeof(E) == 4) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
+    unsigned w;
+    __builtin_memcpy(&w, q, 4);
+    reinterpret_cast<W*>(p)->v = w;
+  } else if constexpr (PV * sizeof(E) == 8) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
+    u32x2 w;
+    __builtin_memcpy(&w, q, 8);
+    reinterpret_cast<W*>(p)->v = w;
+  } else {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) p[v] = q[v];
+  }
+}
+// Pixels of a tile of lanes: lane `pl` of tile `t` has PV pixels from `px` on, those from `p0` on are its own (an image's last lane is
+// moved back so that it loads whole pieces).
+template <int PV>
+struct Px {
+  long long px, p0, P;
+  __device__ __forceinline__ Px(long long first, long long P_) : px(first < P_ - PV ? first : P_ - PV), p0(first), P(P_) {}
+  __device__ __forceinline__ bool own(int v) const { return px + v >= p0; }
+};
+
+// Falling lists of the K best: order keys (fp32) with their classes beside them, or, for 16-bit logits, key and class in one word.
+// Classes come in rising order, so a key equal to one in the list goes behind it.  The median of (upper neighbour, entry, new key) is
+// the entry's new key.
+__device__ __forceinline__ unsigned med3u(unsigned a, unsigned b, unsigned c) { return max(min(a, b), min(max(a, b), c)); }
+template <typename E, int K>
+struct Best {
+  unsigned key[K > 0 ? K : 1];
+  int id[K > 0 ? K : 1];
+  __device__ __forceinline__ Best() {
+#pragma unroll
+    for (int j = 0; j < K; ++j) { key[j] = 0; id[j] = 0; }
+  }
+  __device__ __forceinline__ void add_key(unsigned k, int c) {
+#pragma unroll
+    for (int j = K - 1; j > 0; --j) {
+      id[j] = k > key[j - 1] ? id[j - 1] : k > key[j] ? c : id[j];
+      key[j] = med3u(key[j - 1], key[j], k);
+    }
+    id[0] = k > key[0] ? c : id[0];
+    key[0] = max(key[0], k);
+  }
+  __device__ __forceinline__ void add(E z, int c) { add_key(order_key((float)z), c); }
+  __device__ __forceinline__ float value(int j) const { return key_value(key[j]); }
+  __device__ __forceinline__ int cls(int j) const { return id[j]; }
+};
+template <typename E, int K>
+struct Best16 {
+  unsigned key[K > 0 ? K : 1];
+  __device__ __forceinline__ Best16() {
+#pragma unroll
+    for (int j = 0; j < K; ++j) key[j] = 0;
+  }
+  __device__ __forceinline__ void add_key(unsigned k, int) {
+#pragma unroll
+    for (int j = K - 1; j > 0; --j) key[j] = med3u(key[j - 1], key[j], k);
+    key[0] = max(key[0], k);
+  }
+  __device__ __forceinline__ void add(E z, int c) {
+    constexpr unsigned INF16 = sizeof(E) == 2 && __is_same(E, __bf16) ? 0x7f80u : 0x7c00u;
+    unsigned short h;
+    __builtin_memcpy(&h, &z, 2);
+    unsigned u = h == 0x8000u ? 0u : h;
+    u = (u & 0x7fffu) > INF16 ? 0xffffu : u ^ (u & 0x8000u ? 0xffffu : 0x8000u);
+    add_key(u << 16 | (0xffffu - (unsigned)c), c);
+  }
+  __device__ __forceinline__ float value(int j) const {
+    const unsigned k = key[j] >> 16;
+    const unsigned short h = (unsigned short)(k & 0x8000u ? k ^ 0x8000u : k ^ 0xffffu);
+    E z;
+    __builtin_memcpy(&z, &h, 2);
+    return (float)z;
+  }
+  __device__ __forceinline__ int cls(int j) const { return 0xffff - (int)(key[j] & 0xffffu); }
+};
+template <typename E, int K> struct BestOf { using type = Best16<E, K>; };
+template <int K> struct BestOf<float, K> { using type = Best<float, K>; };
+
+constexpr int PLANE_K = 32, PLANE_CLASSES = 65536;
+
+// SPLIT = 4: a block's four waves share 64 * PV pixels and take a quarter of the classes each (images too small to fill the device).
+template <typename E, int PV, int K, int SPLIT>
+__global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, const LogprobOut o, const long long i0, const int tiles) {
+  using B = typename BestOf<E, K>::type;
+  constexpr int LANES = 256 / SPLIT, UN = 8;
+  __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][3][PV][SPLIT > 1 ? 64 : 1];
+  __shared__ unsigned lists[SPLIT > 1 ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
+  __shared__ int ids[SPLIT > 1 && sizeof(B) > 4 * (K > 0 ? K : 1) ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
+  const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, pl = threadIdx.x & (LANES - 1);
+  const long long i = i0 + blockIdx.x / (unsigned)tiles;
+  const long long first = (long long)(blockIdx.x % (unsigned)tiles) * (LANES * PV) + pl * PV;
+  const Px<PV> px(first, a.p);
+  const E* z = (const E*)a.z + i * a.sn + px.px;
+  const int per = (a.C + SPLIT - 1) / SPLIT, c0 = wv * per, c1 = min(a.C, c0 + per);
+  float m[PV], s[PV], u[PV];
+  B best[PV];
+#pragma unroll
+  for (int v = 0; v < PV; ++v) { m[v] = -INFINITY; s[v] = u[v] = 0.f; }
+  for (int c = c0; c < c1; c += UN) {
+    E q[UN][PV];
+    float x[UN][PV];
+#pragma unroll
+    for (int n = 0; n < UN; ++n) load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, q[n]);
+#pragma unroll
+    for (int n = 0; n < UN; ++n)
+#pragma unroll
+      for (int v = 0; v < PV; ++v) x[n][v] = c + n < c1 ? (float)q[n][v] : -INFINITY;
+#pragma unroll
+    for (int v = 0; v < PV; ++v) {
+      float nm = m[v];
+#pragma unroll
+      for (int n = 0; n < UN; ++n) nm = fmaxf(nm, x[n][v]);
+      const float base = nm == -INFINITY ? 0.f : nm;
+      rescale(s[v], u[v], m[v], base, a.scale2);
+      m[v] = nm;
+#pragma unroll
+      for (int n = 0; n < UN; ++n) {
+        const float d = (x[n][v] - base) * a.scale2, w = exp2_(d);
+        s[v] += w;
+        u[v] += w * fmaxf(d, -300.f);
+      }
+    }
+    if (K > 0) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+        if (c + n < c1) {
+#pragma unroll
+          for (int v = 0; v < PV; ++v) best[v].add(q[n][v], c + n);
+        }
+    }
+  }
+  if (SPLIT > 1) {
+    if (wv > 0) {
+#pragma unroll
+      for (int v = 0; v < PV; ++v) {
+        red[wv - 1][0][v][pl] = m[v];
+        red[wv - 1][1][v][pl] = s[v];
+        red[wv - 1][2][v][pl] = u[v];
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          lists[wv - 1][j][v][pl] = best[v].key[j];
+          if constexpr (sizeof(B) > 4 * (K > 0 ? K : 1)) ids[wv - 1][j][v][pl] = best[v].cls(j);
+        }
+      }
+    }
+    __syncthreads();
+    if (wv > 0) return;
+    for (int w = 0; w < SPLIT - 1; ++w) {
+#pragma unroll
+      for (int v = 0; v < PV; ++v) {
+        const float om = red[w][0][v][pl], nm = fmaxf(m[v], om), base = nm == -INFINITY ? 0.f : nm;
+        float os = red[w][1][v][pl], ou = red[w][2][v][pl];
+        rescale(s[v], u[v], m[v], base, a.scale2);
+        rescale(os, ou, om, base, a.scale2);
+        s[v] += os;
+        u[v] += ou;
+        m[v] = nm;
+        if (K > 0) {
+          for (int j = 0; j < K; ++j) {        // the other waves' classes are higher: equal keys stay behind
+            const unsigned k = lists[w][j][v][pl];
+            int id = 0;
+            if constexpr (sizeof(B) > 4 * (K > 0 ? K : 1)) id = ids[w][j][v][pl];
+            best[v].add_key(k, id);
+          }
+        }
+      }
+    }
+  }
+  if (first >= a.p) return;
+#pragma unroll
+  for (int v = 0; v < PV; ++v) {
+    if (!px.own(v)) continue;
+    const long long r = i * a.p + px.px + v;
+    const long long y = o.label ? o.label[r] : 0;
+    const bool empty = o.label && y == o.ignore, is_class = y >= 0 && y < a.C;
+    const float base = m[v] == -INFINITY ? 0.f : m[v], ls = log2_(s[v]) * LN2;
+    if (empty) void_row(o, r, a.R);
+    else finish_row(o, r, a, base, s[v], u[v], ls, is_class, o.logprob && is_class ? load1(z + y * a.sc + v) : 0.f);
+    const long long ot = i * o.tn + (px.px + v) * o.tp;
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j < o.k) {
+        o.top_ids[ot + j * o.tk] = empty ? -1 : best[v].cls(j);
+        o.top_lp[ot + j * o.tk] = empty || s[v] == 0.f ? -INFINITY : (best[v].value(j) - base) * a.invT - ls;
+      }
+  }
+}
+
 struct LogprobGrad {
   const long long* label;
   long long ignore;
@@ -579,30 +788,88 @@ struct LogprobGrad {
 };
 
 // dz_c = p_c (A + B log p_c) + [c = y] G  with  G = g_logprob / T,  B = -g_entropy / T,  A = (g_lse - g_logprob - g_entropy H) / T
-template <typename E>
-__global__ __launch_bounds__(256) void logprobs_bwd_kernel(const Logits a, const LogprobGrad g) {
-  const int lane = threadIdx.x & 63;
-  const long long waves = (long long)gridDim.x * 4;
-  for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += waves) {
+struct RowGrad {
+  float m, ls, A, B, G;
+  long long y;
+  bool dead;                 // void, or nothing but -inf: no gradient
+  __device__ __forceinline__ RowGrad(const Logits& a, const LogprobGrad& g, long long r) {
+    y = g.label ? g.label[r] : -1;
+    m = g.stats[r];
+    ls = g.stats[a.R + r];
+    dead = (g.label && y == g.ignore) || ls == -INFINITY;
+    G = g.g_logprob && y >= 0 && y < a.C ? g.g_logprob[r] * a.invT : 0.f;
+    B = g.g_entropy ? -g.g_entropy[r] * a.invT : 0.f;
+    A = (g.g_lse ? g.g_lse[r] * a.invT : 0.f) - G + (g.g_entropy ? B * g.entropy[r] : 0.f);
+  }
+  __device__ __forceinline__ float operator()(const Logits& a, float z, int c) const {
+    const float lp = (z - m) * a.invT - ls;
+    float v = exp2_(lp * LOG2E) * (A + B * fmaxf(lp, -200.f));      // exp(-200) = 0 in fp32; 0 * -inf would be NaN
+    if (c == y) v += G;
+    return dead ? 0.f : v;
+  }
+};
+
+// Contiguous classes: G lanes to a row (8, 64) or a block to a segment of SEG chunks a lane; one read, one write, no reductions.
+template <typename E, int G>
+__global__ __launch_bounds__(256) void logprobs_bwd_rows_kernel(const Logits a, const LogprobGrad g, const int segs) {
+  constexpr int V = VEC<E>, SEG = 4;
+  const int l = threadIdx.x % G;
+  const long long step = (long long)gridDim.x * (256 / G), items = a.R * segs;
+  for (long long it = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; it < items; it += step) {
+    long long r = it;
+    int seg = 0;
+    if (segs > 1) {
+      r = items <= 0x7fffffff ? (unsigned)it / (unsigned)segs : it / segs;
+      seg = (int)(it - r * segs);
+    }
+    const RowGrad f(a, g, r);
     const E* z = (const E*)a.z + a.at(r);
     E* dz = (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp);
-    const long long y = g.label ? g.label[r] : -1;
-    const float m = g.stats[r], ls = g.stats[a.R + r];
-    if ((g.label && y == g.ignore) || ls == -INFINITY) {
-      if (!g.accumulate)
-        for (int c = lane; c < a.C; c += 64) store1(dz + c * g.dc, 0.f);
-      continue;
+    for (int q = 0; q < (G == 256 ? SEG : (a.C + G * V - 1) / (G * V)); ++q) {
+      const int c = (G == 256 ? seg * (SEG * G * V) : 0) + (q * G + l) * V;
+      if (c >= a.C) break;
+      float x[V], old[V];
+      const int b = load_chunk<G == 8>(z, c, a.C, x);
+      if (g.accumulate) load_chunk<G == 8>((const E*)dz, c, a.C, old);
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = f(a, x[e], b + e) + (g.accumulate ? old[e] : 0.f);
+      store_chunk(dz, c, b, a.C, x);
     }
-    const bool has = g.g_logprob && y >= 0 && y < a.C;
-    const float G = has ? g.g_logprob[r] * a.invT : 0.f;
-    const float B = g.g_entropy ? -g.g_entropy[r] * a.invT : 0.f;
-    const float A = (g.g_lse ? g.g_lse[r] * a.invT : 0.f) - G + (g.g_entropy ? B * g.entropy[r] : 0.f);
-    for (int c = lane; c < a.C; c += 64) {
-      const float lp = (load1(z + c * a.sc) - m) * a.invT - ls;
-      float v = expf(lp) * (A + B * fmaxf(lp, -200.f));      // exp(-200) = 0 in fp32; 0 * -inf would be NaN
-      if (c == y) v += G;
-      if (g.accumulate) v += load1(dz + c * g.dc);
-      store1(dz + c * g.dc, v);
+  }
+}
+
+// Planes: PV pixels and a slice of the classes to a lane.
+template <typename E, int PV>
+__global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a, const LogprobGrad g, const long long i0, const int tiles,
+                                                                  const int slice) {
+  constexpr int UN = 4;
+  const long long i = i0 + blockIdx.x / (unsigned)tiles;
+  const long long first = (long long)(blockIdx.x % (unsigned)tiles) * (256 * PV) + threadIdx.x * PV;
+  if (first >= a.p) return;
+  const Px<PV> px(first, a.p);
+  const E* z = (const E*)a.z + i * a.sn + px.px;
+  E* dz = (E*)g.dz + i * g.dn + px.px;
+  const RowGrad f0(a, g, i * a.p + px.px), f1(a, g, i * a.p + px.px + PV - 1);
+  const int c0 = blockIdx.y * slice, c1 = min(a.C, c0 + slice);
+  for (int c = c0; c < c1; c += UN) {
+    E q[UN][PV], old[UN][PV];
+#pragma unroll
+    for (int n = 0; n < UN; ++n) {
+      load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, q[n]);
+      if (g.accumulate) load_px<E, PV>(dz + min(c + n, c1 - 1) * g.dc, old[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < UN; ++n) {
+      if (c + n >= c1) break;
+#pragma unroll
+      for (int v = 0; v < PV; ++v) q[n][v] = (E)((v ? f1 : f0)(a, (float)q[n][v], c + n) + (g.accumulate ? (float)old[n][v] : 0.f));
+      if (px.own(0)) {
+        store_px<E, PV>(dz + (c + n) * g.dc, q[n]);
+      } else {
+#pragma unroll
+        for (int v = 1; v < PV; ++v)
+          if (px.own(v)) store1(dz + (c + n) * g.dc + v, (float)q[n][v]);
+      }
     }
   }
 }
@@ -812,6 +1079,8 @@ int row_blocks(long long R) {
 bool logits_ok(const void* z, int type, long long n, long long p, int C, float T) {
   return z && type >= 0 && type <= 2 && n > 0 && p > 0 && C > 0 && p <= (1ll << 40) / n && T > 0.f && T <= 3e38f;
 }
+// rows: contiguous classes; planes: contiguous pixels (of fewer than 2^32 to an image)
+bool layout_ok(int C, long long p, long long sp, long long sc) { return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 32)); }
 bool teacher_ok(const void* ids, int ids64, const void* top, int top_type, int k) {
   return ids && top && (ids64 == 0 || ids64 == 1) && top_type >= 0 && top_type <= 2 && k >= 1 && k <= MAXK;
 }
@@ -836,10 +1105,72 @@ Split split_rows(int type, long long R, int C) {
 }
 int capped(long long blocks, int cap) { return (int)(blocks < cap ? blocks : cap); }
 
+// launch(first image, images): groups of images whose grids stay below 2^32 lanes
+template <typename F>
+void by_images(const Logits& a, long long tiles, F launch) {
+  const long long n = a.R / a.p, most = tiles >= (1ll << 23) ? 1 : (1ll << 23) / tiles;
+  for (long long i = 0; i < n; i += most) launch(i, (int)(n - i < most ? n - i : most));
+}
+
+template <typename E, int PV, int K>
+void logprobs_planes_k(const Logits& a, const LogprobOut& o, hipStream_t stream) {
+  // a wave to every class quarter where whole images to a lane give less than four blocks a compute unit
+  const long long whole = (a.p + 256 * PV - 1) / (256 * PV), quarter = (a.p + 64 * PV - 1) / (64 * PV);
+  if (a.R / a.p * whole >= 1024 || a.C < 16)
+    by_images(a, whole, [&](long long i0, int n) { logprobs_planes_kernel<E, PV, K, 1><<<n * (int)whole, 256, 0, stream>>>(a, o, i0, (int)whole); });
+  else
+    by_images(a, quarter, [&](long long i0, int n) { logprobs_planes_kernel<E, PV, K, 4><<<n * (int)quarter, 256, 0, stream>>>(a, o, i0, (int)quarter); });
+}
+template <typename E>
+void logprobs_planes(const Logits& a, const LogprobOut& o, hipStream_t stream) {
+  constexpr int PV = sizeof(E) == 2 ? 2 : 1;      // two 16-bit pixels to a lane while their lists leave registers for it
+  if (PV == 2 && a.p == 1) {
+    if (o.k <= 16) logprobs_planes_k<E, 1, 16>(a, o, stream);
+    else logprobs_planes_k<E, 1, 32>(a, o, stream);
+  } else if (o.k == 0) logprobs_planes_k<E, PV, 0>(a, o, stream);
+  else if (o.k == 1) logprobs_planes_k<E, PV, 1>(a, o, stream);
+  else if (o.k == 2) logprobs_planes_k<E, PV, 2>(a, o, stream);
+  else if (o.k == 3) logprobs_planes_k<E, PV, 3>(a, o, stream);
+  else if (o.k == 4) logprobs_planes_k<E, PV, 4>(a, o, stream);
+  else if (o.k <= 8) logprobs_planes_k<E, PV, 8>(a, o, stream);
+  else if (o.k <= 16) logprobs_planes_k<E, 1, 16>(a, o, stream);
+  else logprobs_planes_k<E, 1, 32>(a, o, stream);
+}
+
+template <typename E>
+void logprobs_bwd(const Logits& a, const LogprobGrad& g, hipStream_t stream) {
+  if (a.C > 1 && a.sc != 1) {
+    constexpr int PV = sizeof(E) == 2 ? 2 : 1;
+    const int pv = a.p > 1 ? PV : 1;
+    const long long tiles = (a.p + 256 * pv - 1) / (256 * pv);
+    // slices of the classes until there are about eight blocks a compute unit, none shorter than 16 classes
+    const long long blocks = a.R / a.p * tiles;
+    int slices = blocks >= 2048 ? 1 : (int)(2048 / blocks);
+    if (slices > (a.C + 15) / 16) slices = (a.C + 15) / 16;
+    const int slice = (a.C + slices - 1) / slices;
+    by_images(a, tiles * slices, [&](long long i0, int n) {
+      const dim3 grid(n * (unsigned)tiles, (a.C + slice - 1) / slice);
+      if (pv == PV) logprobs_bwd_planes_kernel<E, PV><<<grid, 256, 0, stream>>>(a, g, i0, (int)tiles, slice);
+      else logprobs_bwd_planes_kernel<E, 1><<<grid, 256, 0, stream>>>(a, g, i0, (int)tiles, slice);
+    });
+    return;
+  }
+  if (a.C <= 256) logprobs_bwd_rows_kernel<E, 8><<<capped((a.R + 31) / 32, 16384), 256, 0, stream>>>(a, g, 1);
+  else if (a.C <= 4 * 64 * VEC<E>) logprobs_bwd_rows_kernel<E, 64><<<capped((a.R + 3) / 4, 16384), 256, 0, stream>>>(a, g, 1);
+  else {
+    const int segs = (a.C + 4 * 256 * VEC<E> - 1) / (4 * 256 * VEC<E>);
+    logprobs_bwd_rows_kernel<E, 256><<<capped(a.R * segs, 1 << 20), 256, 0, stream>>>(a, g, segs);
+  }
+}
+
 template <typename E>
 void logprobs_fwd(const Logits& a, const LogprobOut& o, int type, void* scratch, hipStream_t stream) {
   if (a.C > 1 && a.sc != 1) {
-    logprobs_fwd_kernel<E><<<row_blocks(a.R), 256, 0, stream>>>(a, o);
+    if (o.k > PLANE_K || a.C > PLANE_CLASSES) {
+      logprobs_fwd_kernel<E><<<row_blocks(a.R), 256, 0, stream>>>(a, o);
+    } else {
+      logprobs_planes<E>(a, o, stream);
+    }
     return;
   }
   if (a.C <= ROW_CLASSES) {
@@ -894,6 +1225,7 @@ int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p,
                               void* scratch, size_t scratch_bytes, hipStream_t stream) {
   if (!logits_ok(z, type, n, p, C, T) || k < 0 || k > MAXK || k > C || (k && (!top_ids || !top_logprobs)) || (logprob && !label))
     return SEMSEG_EINVAL;
+  if (!layout_ok(C, p, sp, sc)) return SEMSEG_EINVAL;
   const size_t need = semseg_class_logprobs_scratch_bytes(type, n, p, C, sc, k);
   if (need && (!scratch || scratch_bytes < need)) return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
@@ -909,9 +1241,13 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
                               const float* g_logprob, const float* g_entropy, const float* g_lse, void* dz, long long dn,
                               long long dp, long long dc, int accumulate, hipStream_t stream) {
   if (!logits_ok(z, type, n, p, C, T) || !stats || !dz || (g_entropy && !entropy) || (g_logprob && !label)) return SEMSEG_EINVAL;
+  // the gradient is in the logits' form
+  if (!layout_ok(C, p, sp, sc) || !(C == 1 || (sc == 1 ? dc == 1 : dp == 1))) return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
   const LogprobGrad g{label, ignore_index, stats, entropy, g_logprob, g_entropy, g_lse, dz, dn, dp, dc, accumulate};
-  BY_TYPE(type, logprobs_bwd_kernel, <<<row_blocks(a.R), 256, 0, stream>>>(a, g));
+  if (type == SEMSEG_TYPE_F32) logprobs_bwd<float>(a, g, stream);
+  else if (type == SEMSEG_TYPE_BF16) logprobs_bwd<__bf16>(a, g, stream);
+  else logprobs_bwd<_Float16>(a, g, stream);
   return semseg_launch_status();
 }
 

@@ -86,7 +86,7 @@ class _Geom:
         a, b = _groups(sizes[:self.outer], strides[:self.outer]), _groups(sizes[self.outer:], strides[self.outer:])
         if len(a) > 1 or len(b) > 1:
             return None
-        return (a[0][1] if a else 0, b[0][1] if b else 0, s)
+        return (a[0][1] if a else 0, b[0][1] if b and self.p > 1 else 1, s)
 
 
 def _check_logits(z, class_dim, temperature):
