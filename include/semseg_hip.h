@@ -330,8 +330,8 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
  * are not read.  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
  * semseg_distill_scratch_bytes() bytes, nothing needs to be cleared; no atomics, results do not depend on scheduling.
  * _bwd: dz (=|+=) grad_mul * grad_loss (one device float, one per row for NONE, NULL: 1) * d loss / dz.
- * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call. */
-size_t semseg_distill_scratch_bytes(long long n, long long p, int C);
+ * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call; stats may be NULL for rows of contiguous classes up to 2048. */
+size_t semseg_distill_scratch_bytes(int type, long long n, long long p, int C, long long sc);
 int semseg_distill_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp, long long sc,
                        const void* ids, int ids64, const void* top, int top_type, int k, long long in, long long ip,
                        long long ik, long long vn, long long vp, long long vk, const float* weight, float T, int tail,

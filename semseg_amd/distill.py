@@ -59,6 +59,8 @@ class _Geom:
     def __init__(self, z, dim):
         sizes, strides = list(z.shape), list(z.stride())
         self.C, sc = sizes.pop(dim), strides.pop(dim)
+        if self.C > 1 << 30:
+            raise ValueError("at most 2^30 classes, got %d" % self.C)
         self.dim, self.shape = dim, tuple(sizes)
         g = _groups(sizes, strides)
         if len(g) > 2:
@@ -222,13 +224,13 @@ class _Distill(torch.autograd.Function):
         dev = z.device
         with torch.cuda.device(dev):
             stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
-            rows = acc = loss = scratch = None
+            rows = acc = loss = None
             if reduction == "none":
                 rows = torch.empty(g.shape, dtype=torch.float32, device=dev)
             else:
                 acc = torch.empty(2, dtype=torch.float64, device=dev)
                 loss = torch.empty((), dtype=torch.float32, device=dev)
-                scratch = torch.empty(ops.distill_scratch_bytes(*g.geom), dtype=torch.uint8, device=dev)
+            scratch = torch.empty(ops.distill_scratch_bytes(z.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
             ids, ids_s, top, top_s, k, weight = teacher
             ops.distill_fwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, rows, stats, acc, loss,
                             scratch)
@@ -287,7 +289,7 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
         stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
         acc = torch.empty(2, dtype=torch.float64, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        scratch = torch.empty(ops.distill_scratch_bytes(*g.geom), dtype=torch.uint8, device=dev)
+        scratch = torch.empty(ops.distill_scratch_bytes(logits.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
         ids, ids_s, top, top_s, k, weight = teacher
         ops.distill_fwd_bwd(logits, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, stats, acc, loss,
                             grad_scale, out, ds, accumulate, scratch)

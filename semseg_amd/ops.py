@@ -595,8 +595,8 @@ def class_logprobs_bwd(z, geom, strides, label, ignore_index, T, stats, entropy,
                                       _stream()), "class_logprobs_bwd")
 
 
-def distill_scratch_bytes(n, p, C):
-    return int(lib.semseg_distill_scratch_bytes(n, p, C))
+def distill_scratch_bytes(dtype, n, p, C, sc):
+    return int(lib.semseg_distill_scratch_bytes(TYPES[dtype], n, p, C, sc))
 
 
 def _teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction):

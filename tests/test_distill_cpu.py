@@ -94,8 +94,9 @@ def test_the_c_entries_refuse_bad_arguments_without_a_gpu():
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, None, None, None, None, None, p, *s3, 0, None) == -1
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, p, None, p, None, None, p, *s3, 0, None) == -1
     assert lib.semseg_class_logprobs_bwd(p, 0, 1, 4, 8, *s3, None, 255, 1.0, p, None, None, p, None, p, *s3, 0, None) == -1
-    need = lib.semseg_distill_scratch_bytes(1, 4, 8)
-    assert need > 0 and lib.semseg_distill_scratch_bytes(0, 4, 8) == 0
+    need = lib.semseg_distill_scratch_bytes(0, 1, 4, 8, 1)
+    assert need > 0 and lib.semseg_distill_scratch_bytes(0, 0, 4, 8, 1) == 0
+    assert lib.semseg_distill_scratch_bytes(1, 1, 4, 100000, 1) > need
     head = (p, 0, 1, 4, 8, *s3)
     dist = lambda ids=p, i64=0, top=p, tt=0, k=2, T=1.0, red=1, rows=None, stats=p, acc=p, loss=p, scr=p, nb=need: lib.semseg_distill_fwd(  # noqa: E731
         *head, ids, i64, top, tt, k, 0, 2, 1, 0, 2, 1, None, T, 0, red, rows, stats, acc, loss, scr, nb, None)
