@@ -305,12 +305,12 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
  * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
  * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
  * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes), nothing needs to be cleared.
- * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (the ids stay in range, NaN first).
+ * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (its alternatives: NaN and +inf first, by class).
  * semseg_class_logprobs_bwd: dz (=|+=) the gradient from those of logprob, entropy, lse (each may be NULL); 0 for rows that are void
  * or hold only -inf; strides dn, dp, dc; dz has the logits' type, one rounding. */
 enum { SEMSEG_TYPE_F32 = 0, SEMSEG_TYPE_BF16 = 1, SEMSEG_TYPE_F16 = 2 };
 enum { SEMSEG_REDUCE_NONE = 0, SEMSEG_REDUCE_MEAN = 1, SEMSEG_REDUCE_SUM = 2 };
-enum { SEMSEG_CLASS_TOP_MAX = 64 };
+enum { SEMSEG_CLASS_TOP_MAX = 64, SEMSEG_ROW_CLASSES = 2048 };
 size_t semseg_class_logprobs_scratch_bytes(int type, long long n, long long p, int C, long long sc, int k);
 int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp,
                               long long sc, const long long* label, long long ignore_index, float T, int k, float* logprob,
@@ -330,7 +330,8 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
  * are not read.  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
  * semseg_distill_scratch_bytes() bytes, nothing needs to be cleared; no atomics, results do not depend on scheduling.
  * _bwd: dz (=|+=) grad_mul * grad_loss (one device float, one per row for NONE, NULL: 1) * d loss / dz.
- * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call; stats may be NULL for rows of contiguous classes up to 2048. */
+ * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call; stats may be NULL for rows of contiguous classes up to
+ * SEMSEG_ROW_CLASSES. */
 size_t semseg_distill_scratch_bytes(int type, long long n, long long p, int C, long long sc);
 int semseg_distill_fwd(const void* z, int type, long long n, long long p, int C, long long sn, long long sp, long long sc,
                        const void* ids, int ids64, const void* top, int top_type, int k, long long in, long long ip,

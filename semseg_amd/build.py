@@ -8,7 +8,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libsemseg_hip.so")
 SOURCES = ["conv_igemm.hip", "conv_wgrad.hip", "stem.hip", "bn.hip", "pool_interp.hip", "ce_head.hip", "psamask.hip",
-           "psa_ops.hip", "infer.hip", "optim.hip", "augment.hip", "winograd.hip", "gemm_bf16split.hip", "xchg.hip", "plan.hip", "class_probs.hip"]
+           "psa_ops.hip", "infer.hip", "optim.hip", "augment.hip", "winograd.hip", "gemm_bf16split.hip", "xchg.hip", "plan.hip", "class_logprobs.hip", "distill.hip"]
 HEADER = os.path.join(HERE, "..", "include", "semseg_hip.h")
 THUNKS = os.path.join(CSRC, "plan_thunks.inc")
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 — some of their forms have given wrong results on this hardware now and then, with no

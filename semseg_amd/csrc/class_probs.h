@@ -1,0 +1,238 @@
+// Class probabilities of logits: what class_logprobs.hip (log probabilities, entropy, alternatives) and distill.hip (distillation) share.
+//
+// A row is one pixel (or token) with C logits.  Rows are addressed as r = i * p + j, class c of row r at z[i * sn + j * sp + c * sc]
+// (element strides): sc = 1 is the engine's pixel-major score buffer ("rows"), sp = 1 a model's [N, C, H, W] output ("planes").
+//
+// With m = max_c z_c, d_c = (z_c - m) / T, S = sum exp(d_c):
+//   lse = m / T + log S      log p_c = d_c - log S      entropy = log S - (sum exp(d_c) d_c) / S
+// The maximum is subtracted from the logits themselves, before the temperature: the difference of two close fp32 values is exact, a
+// logsumexp rounded to fp32 and subtracted later is not (at |z| ~ 1e3 it would cost 6e-5 of every log probability).  All sums are fp32
+// over fp32 terms (16-bit logits are widened exactly), losses are summed over rows in fp64; results are rounded to 16 bits only where a
+// gradient is stored in the logits' type.
+#pragma once
+#include "common.h"
+#include "../../include/semseg_hip.h"
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr int MAXK = SEMSEG_CLASS_TOP_MAX;
+
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __bf16* p) { return (float)*p; }
+__device__ __forceinline__ float load1(const _Float16* p) { return (float)*p; }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__bf16* p, float v) { *p = (__bf16)v; }
+__device__ __forceinline__ void store1(_Float16* p, float v) { *p = (_Float16)v; }
+
+// Order of the alternatives as unsigned integers: larger logit first, NaN above everything, -0 = +0.  Never 0.
+__device__ __forceinline__ unsigned order_key(float z) {
+  const unsigned u = __float_as_uint(z + 0.f);
+  const unsigned k = u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+  return z != z ? 0xfffffffeu : k;
+}
+// ... with the class as the second criterion: the lowest one first
+__device__ __forceinline__ unsigned long long pair_key(float z, int c) {
+  return ((unsigned long long)order_key(z) << 32) | (unsigned)~c;
+}
+
+// ---- reductions over groups of G = 8 or 64 neighbouring lanes: data-parallel moves inside a row of 16 lanes, swaps of rows beyond
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
+constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
+template <int G, typename T, typename F>
+__device__ __forceinline__ T group_reduce(T v, F f) {
+  static_assert(sizeof(T) == 4, "");
+  const auto bits = [](T x) { return __builtin_bit_cast(unsigned, x); };
+  const auto val = [](unsigned x) { return __builtin_bit_cast(T, x); };
+  v = f(v, val(dpp<XOR1>(bits(v))));
+  v = f(v, val(dpp<XOR2>(bits(v))));
+  v = f(v, val(dpp<HALF_MIRROR>(bits(v))));
+  if (G == 64) {
+    v = f(v, val(dpp<MIRROR>(bits(v))));
+    // both operands v: the odd rows (the upper half) of the one and the even rows (the lower half) of the other change places
+    const auto r = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    v = f(val(r[0]), val(r[1]));
+    const auto h = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = f(val(h[0]), val(h[1]));
+  }
+  return v;
+}
+template <int G> __device__ __forceinline__ float group_max(float v) { return group_reduce<G>(v, [](float a, float b) { return fmaxf(a, b); }); }
+template <int G> __device__ __forceinline__ float group_sum(float v) { return group_reduce<G>(v, [](float a, float b) { return a + b; }); }
+template <int G> __device__ __forceinline__ unsigned group_umax(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a > b ? a : b; }); }
+template <int G> __device__ __forceinline__ unsigned group_umin(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a < b ? a : b; }); }
+// by two reductions: the high words, then the low words of those that have the highest
+__device__ __forceinline__ unsigned long long wave_max64(unsigned long long v) {
+  const unsigned hi = group_umax<64>((unsigned)(v >> 32));
+  const unsigned lo = group_umax<64>((unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
+  return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_(float v) { return __builtin_amdgcn_logf(v); }
+
+// ---- 16 bytes of logits at an element's own alignment: rows of odd lengths start anywhere, and global loads and stores of this hardware
+// need no more than that
+template <typename E> constexpr int VEC = 16 / (int)sizeof(E);
+template <typename E>
+using Vec = E __attribute__((ext_vector_type(16 / sizeof(E))));
+template <typename E>
+struct __attribute__((packed, aligned(alignof(E)))) Raw { u32x4 v; };
+template <typename E>
+__device__ __forceinline__ void load_vec(const E* p, float (&x)[VEC<E>]) {
+  const Vec<E> q = __builtin_bit_cast(Vec<E>, reinterpret_cast<const Raw<E>*>(p)->v);
+#pragma unroll
+  for (int e = 0; e < VEC<E>; ++e) x[e] = (float)q[e];
+}
+template <typename E>
+__device__ __forceinline__ void store_vec(E* p, const float (&x)[VEC<E>]) {
+  Vec<E> q;
+#pragma unroll
+  for (int e = 0; e < VEC<E>; ++e) q[e] = (E)x[e];
+  reinterpret_cast<Raw<E>*>(p)->v = __builtin_bit_cast(u32x4, q);
+}
+// VEC classes of a row of C from class s on; what lies beyond the row is -inf and not read.  Returns the class of x[0]: the row's last
+// chunk is loaded from C - VEC, its classes below s (another lane has them) made -inf too.  SHORT: C may be less than VEC.
+template <bool SHORT = false, typename E>
+__device__ __forceinline__ int load_chunk(const E* z, int s, int C, float (&x)[VEC<E>]) {
+  constexpr int V = VEC<E>;
+  if (!SHORT || C >= V) {
+    const int b = min(s, C - V);
+    load_vec(z + b, x);
+    if (b != s) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[e] = b + e >= s ? x[e] : -INFINITY;
+    }
+    return b;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e) x[e] = s + e < C ? load1(z + s + e) : -INFINITY;
+  return s;
+}
+template <typename E>
+__device__ __forceinline__ void store_chunk(E* z, int s, int b, int C, const float (&x)[VEC<E>]) {
+  if (s + VEC<E> <= C) {
+    store_vec(z + s, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC<E>; ++e)
+      if (b + e >= s && b + e < C) store1(z + b + e, x[e]);
+  }
+}
+
+template <int G, typename E>
+__device__ __forceinline__ void zero_row(E* dz, int l, int C) {
+  float x[VEC<E>];
+#pragma unroll
+  for (int e = 0; e < VEC<E>; ++e) x[e] = 0.f;
+  for (int c = l * VEC<E>; c < C; c += G * VEC<E>) store_chunk(dz, c, C < VEC<E> ? c : min(c, C - VEC<E>), C, x);
+}
+
+// i * s0 + j * s1 of row r = i * p + j; 64-bit divisions (~150 instructions) are kept out of the usual cases
+__device__ __forceinline__ long long row_at(long long r, long long p, long long R, long long s0, long long s1) {
+  if (p == R) return r * s1;
+  if (R <= 0x7fffffff) {
+    const unsigned i = (unsigned)r / (unsigned)p;
+    return i * s0 + ((unsigned)r - i * (unsigned)p) * s1;
+  }
+  return (r / p) * s0 + (r % p) * s1;
+}
+
+struct Logits {
+  const void* z;
+  long long R, p, sn, sp, sc;
+  int C;
+  float invT, scale2;      // 1 / T, log2(e) / T
+  __device__ __forceinline__ long long at(long long r) const { return row_at(r, p, R, sn, sp); }
+};
+
+// s, u taken about `from` become sums about `to` >= from (u's terms carry a factor d); an empty sum may come from -inf
+__device__ __forceinline__ void rescale(float& s, float& u, float from, float to, float scale2) {
+  const float d = (from - to) * scale2, f = exp2_(d);
+  u = (u + s * fmaxf(d, -300.f)) * f;
+  s = s * f;
+}
+
+// ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane
+template <typename E, int PV>
+__device__ __forceinline__ void load_px(const E* p, E (&q)[PV]) {
+  if constexpr (PV * sizeof(E) == 4) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
+    const unsigned w = reinterpret_cast<const W*>(p)->v;
+    __builtin_memcpy(q, &w, 4);
+  } else if constexpr (PV * sizeof(E) == 8) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
+    const u32x2 w = reinterpret_cast<const W*>(p)->v;
+    __builtin_memcpy(q, &w, 8);
+  } else {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) q[v] = p[v];
+  }
+}
+template <typename E, int PV>
+__device__ __forceinline__ void store_px(E* p, const E (&q)[PV]) {
+  if constexpr (PV * sizeof(E) == 4) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
+    unsigned w;
+    __builtin_memcpy(&w, q, 4);
+    reinterpret_cast<W*>(p)->v = w;
+  } else if constexpr (PV * sizeof(E) == 8) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
+    u32x2 w;
+    __builtin_memcpy(&w, q, 8);
+    reinterpret_cast<W*>(p)->v = w;
+  } else {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) p[v] = q[v];
+  }
+}
+// Pixels of a tile of lanes: lane `pl` of tile `t` has PV pixels from `px` on, those from `p0` on are its own (an image's last lane is
+// moved back so that it loads whole pieces).
+template <int PV>
+struct Px {
+  long long px, p0, P;
+  __device__ __forceinline__ Px(long long first, long long P_) : px(first < P_ - PV ? first : P_ - PV), p0(first), P(P_) {}
+  __device__ __forceinline__ bool own(int v) const { return px + v >= p0; }
+};
+
+// ---- host side
+inline bool logits_ok(const void* z, int type, long long n, long long p, int C, float T) {
+  return z && type >= 0 && type <= 2 && n > 0 && p > 0 && C > 0 && C <= (1 << 30) && p <= (1ll << 40) / n && T > 0.f && T <= 3e38f;
+}
+// rows: contiguous classes; planes: contiguous pixels (of fewer than 2^31 to an image)
+inline bool layout_ok(int C, long long p, long long sp, long long sc) { return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 31)); }
+inline Logits logits_of(const void* z, long long n, long long p, int C, long long sn, long long sp, long long sc, float T) {
+  return Logits{z, n * p, p, sn, sp, sc, C, 1.f / T, LOG2E / T};
+}
+
+// Slices of a row of more classes than ROW_CLASSES: none with 512 rows or more (two blocks a compute unit), else about 1024 blocks in
+// all, a slice no shorter than 4096 classes.
+constexpr int ROW_CLASSES = SEMSEG_ROW_CLASSES;      // held in registers up to here
+struct Split { int nsplit, slice, join; };
+inline Split split_rows(int type, long long R, int C) {
+  const int v = type == SEMSEG_TYPE_F32 ? 4 : 8;
+  if (C <= ROW_CLASSES) return Split{1, C, 1};
+  long long n = R >= 512 ? 1 : 1024 / R;
+  if (n > 64) n = 64;
+  if (n > (C + 4095) / 4096) n = (C + 4095) / 4096;
+  const int slice = (int)(((C + n - 1) / n + v - 1) / v * v);
+  const int iters = (slice + 256 * v - 1) / (256 * v);
+  return Split{(C + slice - 1) / slice, slice, (iters + 127) / 128};
+}
+inline int capped(long long blocks, int cap) { return (int)(blocks < cap ? blocks : cap); }
+
+// launch(first image, images): groups of images whose grids stay below 2^32 lanes
+template <typename F>
+void by_images(const Logits& a, long long tiles, F launch) {
+  const long long n = a.R / a.p, most = tiles >= (1ll << 23) ? 1 : (1ll << 23) / tiles;
+  for (long long i = 0; i < n; i += most) launch(i, (int)(n - i < most ? n - i : most));
+}
+
+#define BY_TYPE(type, F, ...)                                  \
+  do {                                                         \
+    if (type == SEMSEG_TYPE_F32) F<float>(__VA_ARGS__);        \
+    else if (type == SEMSEG_TYPE_BF16) F<__bf16>(__VA_ARGS__); \
+    else F<_Float16>(__VA_ARGS__);                             \
+  } while (0)
+
+}  // namespace

@@ -1,5 +1,5 @@
 """Class probabilities of logits on tensors: log probabilities of given classes with entropy and top alternatives, and distillation from
-a teacher's stored top logits.  The kernels are csrc/class_probs.hip (include/semseg_hip.h); nothing here computes.
+a teacher's stored top logits.  The kernels are csrc/class_logprobs.hip and csrc/distill.hip (include/semseg_hip.h); nothing here computes.
 
     top = class_logprobs(teacher_logits, topk=8)                          # what a teacher answers: keep top.top_ids, top.top_logprobs
     loss = distill_loss(student_logits, top.top_ids, top.top_logprobs, temperature=4.0)
@@ -12,6 +12,7 @@ neither form is refused.  Every gradient is a new tensor in the logits' type; do
 
 Work is launched on the current stream of the logits' device and never waits for it; workspaces come from torch's allocator call by
 call, so calls on several streams and captured graphs share none.  Outputs do not depend on scheduling (no atomics)."""
+import contextlib
 from typing import NamedTuple, Optional
 
 import torch
@@ -80,6 +81,10 @@ class _Geom:
             return torch.empty(self.shape + (size,), dtype=dtype, device=device).movedim(-1, self.dim)
         return torch.empty(self.shape[:self.dim] + (size,) + self.shape[self.dim:], dtype=dtype, device=device)
 
+    def dense(self, size):
+        """Strides (sn, sp, s of `dim`) of what empty(size) gives."""
+        return (self.p * size, size, 1) if self.by_rows else (size * self.p, 1, self.p)
+
     def strides_of(self, t):
         """(sn, sp, s of `dim`) of a tensor with these rows; None where its rows do not split the same way."""
         sizes, strides = list(t.shape), list(t.stride())
@@ -122,28 +127,36 @@ def _on_gpu(z):
         raise RuntimeError("semseg_amd runs on the MI355X only: move the logits to cuda (there is no CPU fallback)")
 
 
+def _on_device(z):
+    """The logits' device as the current one (nothing to do where it is: entering a device costs as much as a launch)."""
+    return contextlib.nullcontext() if z.device.index == torch.cuda.current_device() else torch.cuda.device(z.device)
+
+
 # ---------------------------------------------------------------------------------------------
 # log probabilities, entropy, top alternatives
 # ---------------------------------------------------------------------------------------------
+def _logprobs(z, g, label, ignore_index, temperature, k, stats):
+    dev, ids, tlp, ts = z.device, None, None, (0, 0, 0)
+    logprob = None if label is None else torch.empty(g.shape, dtype=torch.float32, device=dev)
+    entropy, lse = (torch.empty(g.shape, dtype=torch.float32, device=dev) for _ in range(2))
+    if k:
+        ids, tlp, ts = g.empty(k, torch.int32, dev), g.empty(k, torch.float32, dev), g.dense(k)
+    need = ops.class_logprobs_scratch_bytes(z.dtype, *g.geom, g.strides[2], k)
+    scratch = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ops.class_logprobs_fwd(z, g.geom, g.strides, label, ignore_index, temperature, k, logprob, entropy, lse, stats, ids, tlp, ts, scratch)
+    return logprob, entropy, lse, ids, tlp
+
+
 class _Logprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, g, label, ignore_index, temperature, k):
-        with torch.cuda.device(z.device):
-            new = lambda: torch.empty(g.shape, dtype=torch.float32, device=z.device)  # noqa: E731
-            logprob, entropy, lse = (None if label is None else new()), new(), new()
-            stats = torch.empty((2,) + g.shape, dtype=torch.float32, device=z.device) if ctx.needs_input_grad[0] else None
-            ids = tlp = None
-            ts = (0, 0, 0)
-            if k:
-                ids, tlp = g.empty(k, torch.int32, z.device), g.empty(k, torch.float32, z.device)
-                ts = g.strides_of(ids)
-            need = ops.class_logprobs_scratch_bytes(z.dtype, *g.geom, g.strides[2], k)
-            scratch = torch.empty(need, dtype=torch.uint8, device=z.device) if need else None
-            ops.class_logprobs_fwd(z, g.geom, g.strides, label, ignore_index, temperature, k, logprob, entropy, lse, stats, ids, tlp, ts,
-                                   scratch)
+        with _on_device(z):
+            stats = torch.empty((2,) + g.shape, dtype=torch.float32, device=z.device)
+            logprob, entropy, lse, ids, tlp = _logprobs(z, g, label, ignore_index, temperature, k, stats)
         ctx.save_for_backward(z, label, stats, entropy)
         ctx.g, ctx.ignore_index, ctx.temperature = g, ignore_index, temperature
-        ctx.mark_non_differentiable(*[t for t in (ids, tlp) if t is not None])
+        if k:
+            ctx.mark_non_differentiable(ids, tlp)
         ctx.set_materialize_grads(False)
         return logprob, entropy, lse, ids, tlp
 
@@ -152,13 +165,13 @@ class _Logprobs(torch.autograd.Function):
     def backward(ctx, g_logprob, g_entropy, g_lse, *_):
         z, label, stats, entropy = ctx.saved_tensors
         g = ctx.g
-        with torch.cuda.device(z.device):
+        with _on_device(z):
             dz = g.empty(g.C, z.dtype, z.device)
             if g_logprob is None and g_entropy is None and g_lse is None:
                 return dz.zero_(), None, None, None, None, None
             gs = [None if t is None else t.contiguous() for t in (g_logprob, g_entropy, g_lse)]
             ops.class_logprobs_bwd(z, g.geom, g.strides, label, ctx.ignore_index, ctx.temperature, stats, entropy, *gs, dz,
-                                   g.strides_of(dz))
+                                   g.dense(g.C))
         return dz, None, None, None, None, None
 
 
@@ -176,7 +189,10 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255
     if isinstance(topk, bool) or not isinstance(topk, int) or not 0 <= topk <= min(TOP_MAX, g.C):
         raise ValueError("topk must be a whole number of [0, min(%d, classes = %d)], got %r" % (TOP_MAX, g.C, topk))
     _on_gpu(logits)
-    return ClassLogprobs(*_Logprobs.apply(logits, g, label, int(ignore_index), float(temperature), topk))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return ClassLogprobs(*_Logprobs.apply(logits, g, label, int(ignore_index), float(temperature), topk))
+    with _on_device(logits):
+        return ClassLogprobs(*_logprobs(logits, g, label, int(ignore_index), float(temperature), topk, None))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -218,25 +234,28 @@ def _check_teacher(logits, top_ids, top_values, temperature, weight, class_dim, 
     return g, (ids, ids_s, top, top_s, k, weight)
 
 
+def _distill(z, g, teacher, temperature, tail, reduction):
+    dev, rows, acc, loss = z.device, None, None, None
+    stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
+    if reduction == "none":
+        rows = torch.empty(g.shape, dtype=torch.float32, device=dev)
+    else:
+        acc, loss = torch.empty(2, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
+    scratch = torch.empty(ops.distill_scratch_bytes(z.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
+    ids, ids_s, top, top_s, k, weight = teacher
+    ops.distill_fwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, rows, stats, acc, loss, scratch)
+    return (rows if loss is None else loss), stats, acc
+
+
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, g, teacher, temperature, tail, reduction):
-        dev = z.device
-        with torch.cuda.device(dev):
-            stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
-            rows = acc = loss = None
-            if reduction == "none":
-                rows = torch.empty(g.shape, dtype=torch.float32, device=dev)
-            else:
-                acc = torch.empty(2, dtype=torch.float64, device=dev)
-                loss = torch.empty((), dtype=torch.float32, device=dev)
-            scratch = torch.empty(ops.distill_scratch_bytes(z.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
-            ids, ids_s, top, top_s, k, weight = teacher
-            ops.distill_fwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, rows, stats, acc, loss,
-                            scratch)
+        with _on_device(z):
+            loss, stats, acc = _distill(z, g, teacher, temperature, tail, reduction)
+        ids, ids_s, top, top_s, k, weight = teacher
         ctx.save_for_backward(z, ids, top, weight, stats, acc)
         ctx.g, ctx.how = g, (ids_s, top_s, k, temperature, tail, reduction)
-        return rows if loss is None else loss
+        return loss
 
     @staticmethod
     @once_differentiable
@@ -244,10 +263,10 @@ class _Distill(torch.autograd.Function):
         z, ids, top, weight, stats, acc = ctx.saved_tensors
         g = ctx.g
         ids_s, top_s, k, temperature, tail, reduction = ctx.how
-        with torch.cuda.device(z.device):
+        with _on_device(z):
             dz = g.empty(g.C, z.dtype, z.device)
             ops.distill_bwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, stats, acc,
-                            grad.contiguous(), 1.0, dz, g.strides_of(dz))
+                            grad.contiguous(), 1.0, dz, g.dense(g.C))
         return dz, None, None, None, None, None
 
 
@@ -261,7 +280,10 @@ def distill_loss(logits, top_ids, top_logits, temperature=1.0, tail=False, weigh
     A negative id is an absent entry, a row without entries counts with loss 0; an id that is no class makes the loss NaN.
     weight: fp32 per row; rows of weight 0 are not read.  reduction: "mean" (over the weights' sum; NaN where that is 0), "sum", "none"."""
     g, teacher = _check_teacher(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum", "none"))
-    return _Distill.apply(logits, g, teacher, float(temperature), bool(tail), reduction)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _Distill.apply(logits, g, teacher, float(temperature), bool(tail), reduction)
+    with _on_device(logits):
+        return _distill(logits, g, teacher, float(temperature), bool(tail), reduction)[0]
 
 
 def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, weight=None, class_dim=1, reduction="mean",
@@ -274,7 +296,7 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
     if out is None:
         if accumulate:
             raise ValueError("accumulate=True needs out")
-        out = g.empty(g.C, logits.dtype, dev)
+        out, ds = g.empty(g.C, logits.dtype, dev), g.dense(g.C)
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
             raise ValueError("out must have the logits' shape, type and device")
@@ -282,13 +304,14 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
             raise ValueError("out must not require a gradient")
         if any(_overlap(out, t) for t in (logits, top_ids, top_logits, weight) if t is not None):
             raise ValueError("out shares memory with an input")
-    ds = g.strides_of(out)
-    if ds is None or not (ds[2] == 1 if g.by_rows and g.C > 1 else g.C == 1 or ds[1] == 1 or g.p == 1) or 0 in out.stride():
-        raise ValueError("out of strides %s does not have the logits' layout" % (tuple(out.stride()),))
-    with torch.cuda.device(dev), torch.no_grad():
-        stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
-        acc = torch.empty(2, dtype=torch.float64, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
+        ds = g.strides_of(out)
+        if ds is None or not (ds[2] == 1 if g.by_rows and g.C > 1 else g.C == 1 or ds[1] == 1) or any(
+                st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
+            raise ValueError("out of strides %s does not have the logits' layout" % (tuple(out.stride()),))
+    with _on_device(logits):
+        # rows that fit registers need no statistics kept for a second pass
+        stats = None if g.by_rows and g.C <= ops.ROW_CLASSES else torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
+        acc, loss = torch.empty(2, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
         scratch = torch.empty(ops.distill_scratch_bytes(logits.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
         ids, ids_s, top, top_s, k, weight = teacher
         ops.distill_fwd_bwd(logits, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, stats, acc, loss,

@@ -572,6 +572,7 @@ def ce_head_bwd(scores, ld, label, lse, acc2, grad_loss, grad_mul, dscores, lddz
 # class probabilities: log probabilities, entropy, top alternatives; distillation (semseg_amd.distill is the tensor-level interface)
 # ---------------------------------------------------------------------------------------------
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ROW_CLASSES = 2048      # SEMSEG_ROW_CLASSES
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
