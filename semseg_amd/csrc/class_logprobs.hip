@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
   for (long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.R; r += waves) {
     const E* z = (const E*)a.z + a.at(r);
     const long long y = o.label ? o.label[r] : 0;
-    const long long ot = row_at(r, a.p, a.R, o.tn, o.tp);
+    const long long ot = row_at(a, r, o.tn, o.tp);
     if (o.label && y == o.ignore) {            // a void row is not read
       if (lane == 0) void_row(o, r, a.R);
       if (lane < o.k) {
@@ -80,20 +80,22 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
   }
 }
 
-// Rows of at most 2048 contiguous classes: G lanes (8 up to 256 classes, 64 beyond) hold a row in registers, NV chunks of 16 bytes each,
-// so it is read once and its maximum, sums and alternatives are reductions over registers and a few data-parallel moves.
+// Rows of at most 2048 contiguous classes: G lanes (4 up to 160 classes, 8 up to 256, 64 beyond) hold a row in registers, NV chunks of
+// 16 bytes each, so it is read once and its maximum, sums and alternatives are reductions over registers and a few data-parallel moves.
+// Few lanes to a row, because most of an alternative's instructions cost the same whatever they serve: with 4 lanes 16 rows a wave.
 // An alternative is one round: the lanes' chunk maxima, their largest, the lowest class that has it, that class taken out and its chunk's
 // maximum renewed.  The chunks lie in LDS too, where a lane reads the one that it needs by its number (selecting it from registers, and
 // changing it there, took twice the instructions: 57600 x 150, 8 alternatives: 22.9 us).
 template <typename E, int G, int NV, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, const LogprobOut o) {
   constexpr int V = VEC<E>;
+  constexpr bool SHORT = G < 64 && NV == 1;
   __shared__ __attribute__((aligned(16))) float keep[TOP ? NV : 1][TOP ? 256 : 1][V];
   const int l = threadIdx.x % G;
   const long long step = (long long)gridDim.x * (256 / G);
   for (long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; r < a.R; r += step) {
     const long long y = o.label ? o.label[r] : 0;
-    const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+    const long long ot = o.k ? row_at(a, r, o.tn, o.tp) : 0;
     if (o.label && y == o.ignore) {
       if (l == 0) void_row(o, r, a.R);
       for (int j = l; j < o.k; j += G) {
@@ -105,8 +107,7 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
     const E* z = (const E*)a.z + a.at(r);
     float x[NV][V];
     int b[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) b[i] = load_chunk<G == 8 && NV == 1>(z, (i * G + l) * V, a.C, x[i]);
+    load_chunks<NV, SHORT>(z, l * V, G * V, a.C, x, b);
     float zy = 0.f;
     const bool is_class = y >= 0 && y < a.C;
     if (l == 0 && o.logprob && is_class) zy = load1(z + y);
@@ -151,6 +152,8 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
 #pragma unroll
       for (int e = 0; e < V; e += 4) *reinterpret_cast<f32x4*>(&keep[i][threadIdx.x][e]) = f32x4{x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3]};
     }
+    int kid = 0;
+    float kv = 0.f;
     for (int j = 0; j < o.k; ++j) {
       float best = cm[0];
 #pragma unroll
@@ -168,7 +171,7 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
 #pragma unroll
         for (int e = V - 1; e >= 0; --e) at = y[e] == best ? e : at;
         const int first = (ch * G + l) * V;
-        c = (unsigned)((G == 8 && NV == 1 && a.C < V ? first : min(first, a.C - V)) + at);
+        c = (unsigned)((SHORT && a.C < V ? first : min(first, a.C - V)) + at);
       }
       const unsigned lowest = group_umin<G>(c);
       if (c == lowest) {
@@ -178,8 +181,14 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
 #pragma unroll
         for (int i = 0; i < NV; ++i) cm[i] = i == ch ? nm : cm[i];
         keep[ch][threadIdx.x][at] = NAN;
-        o.top_ids[ot + j * o.tk] = (int)c;
-        o.top_lp[ot + j * o.tk] = s == 0.f ? -INFINITY : (best - base) * a.invT - ls;
+      }
+      // G alternatives, one to a lane, are written together
+      const int jl = j & (G - 1);
+      kid = jl == l ? (int)lowest : kid;
+      kv = jl == l ? best : kv;
+      if ((jl == G - 1 || j == o.k - 1) && l <= jl) {
+        o.top_ids[ot + (j - jl + l) * o.tk] = kid;
+        o.top_lp[ot + (j - jl + l) * o.tk] = s == 0.f ? -INFINITY : (kv - base) * a.invT - ls;
       }
     }
   }
@@ -214,7 +223,7 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
   const int sp = (int)(blockIdx.x % (unsigned)t.nsplit);
   const long long r = t.r0 + blockIdx.x / (unsigned)t.nsplit;
   const long long y = o.label ? o.label[r] : 0;
-  const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+  const long long ot = o.k ? row_at(a, r, o.tn, o.tp) : 0;
   if (o.label && y == o.ignore) {      // with several slices the joining kernel writes the row
     if (t.nsplit == 1) {
       if (tid == 0) void_row(o, r, a.R);
@@ -404,7 +413,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const Logits a, const
   const int lane = threadIdx.x;
   const long long r = t.r0 + blockIdx.x;
   const long long y = o.label ? o.label[r] : 0;
-  const long long ot = o.k ? row_at(r, a.p, a.R, o.tn, o.tp) : 0;
+  const long long ot = o.k ? row_at(a, r, o.tn, o.tp) : 0;
   if (o.label && y == o.ignore) {
     if (lane == 0) void_row(o, r, a.R);
     if (lane < o.k) {
@@ -445,73 +454,56 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const Logits a, const
   }
 }
 
-// Falling lists of the K best: order keys (fp32) with their classes beside them, or, for 16-bit logits, key and class in one word.
-// Classes come in rising order, so a key equal to one in the list goes behind it.  The median of (upper neighbour, entry, new key) is
-// the entry's new key.
+// Falling lists of the K best: order keys with their classes beside them (fp32), or key and class in one word: an fp32 value that was
+// bf16 (fp16) leaves the 16 (13) last bits of its key to the class, counted down.  Classes come in rising order, so a key equal to one in
+// the list goes behind it.  The median of (upper neighbour, entry, new key) is the entry's new key.  NaN is not looked for here: its row's
+// sum tells of it, and its alternatives are taken once more.
 __device__ __forceinline__ unsigned med3u(unsigned a, unsigned b, unsigned c) { return max(min(a, b), min(max(a, b), c)); }
+__device__ __forceinline__ unsigned plain_key(float z) {
+  const unsigned u = __float_as_uint(z + 0.f);
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+template <typename E> constexpr unsigned CLASS_BITS = 0;
+template <> constexpr unsigned CLASS_BITS<__bf16> = 0xffffu;
+template <> constexpr unsigned CLASS_BITS<_Float16> = 0x1fffu;
 template <typename E, int K>
 struct Best {
+  static constexpr unsigned BITS = CLASS_BITS<E>;
   unsigned key[K > 0 ? K : 1];
-  int id[K > 0 ? K : 1];
+  int id[K > 0 && BITS == 0 ? K : 1];
   __device__ __forceinline__ Best() {
 #pragma unroll
-    for (int j = 0; j < K; ++j) { key[j] = 0; id[j] = 0; }
+    for (int j = 0; j < K; ++j) {
+      key[j] = 0;
+      if constexpr (BITS == 0) id[j] = 0;
+    }
   }
   __device__ __forceinline__ void add_key(unsigned k, int c) {
 #pragma unroll
     for (int j = K - 1; j > 0; --j) {
-      id[j] = k > key[j - 1] ? id[j - 1] : k > key[j] ? c : id[j];
+      if constexpr (BITS == 0) id[j] = k > key[j - 1] ? id[j - 1] : k > key[j] ? c : id[j];
       key[j] = med3u(key[j - 1], key[j], k);
     }
-    id[0] = k > key[0] ? c : id[0];
+    if constexpr (BITS == 0) id[0] = k > key[0] ? c : id[0];
     key[0] = max(key[0], k);
   }
-  __device__ __forceinline__ void add(E z, int c) { add_key(order_key((float)z), c); }
-  __device__ __forceinline__ float value(int j) const { return key_value(key[j]); }
-  __device__ __forceinline__ int cls(int j) const { return id[j]; }
+  __device__ __forceinline__ void add(float z, int c) { add_key((plain_key(z) & ~BITS) | (BITS - (BITS ? (unsigned)c : 0u)), c); }
+  __device__ __forceinline__ float value(int j) const { return key_value(BITS == 0 ? key[j] : key[j] & 0x80000000u ? key[j] & ~BITS : key[j] | BITS); }
+  __device__ __forceinline__ int cls(int j) const { return BITS ? (int)(BITS - (key[j] & BITS)) : id[j]; }
 };
-template <typename E, int K>
-struct Best16 {
-  unsigned key[K > 0 ? K : 1];
-  __device__ __forceinline__ Best16() {
-#pragma unroll
-    for (int j = 0; j < K; ++j) key[j] = 0;
-  }
-  __device__ __forceinline__ void add_key(unsigned k, int) {
-#pragma unroll
-    for (int j = K - 1; j > 0; --j) key[j] = med3u(key[j - 1], key[j], k);
-    key[0] = max(key[0], k);
-  }
-  __device__ __forceinline__ void add(E z, int c) {
-    constexpr unsigned INF16 = sizeof(E) == 2 && __is_same(E, __bf16) ? 0x7f80u : 0x7c00u;
-    unsigned short h;
-    __builtin_memcpy(&h, &z, 2);
-    unsigned u = h == 0x8000u ? 0u : h;
-    u = (u & 0x7fffu) > INF16 ? 0xffffu : u ^ (u & 0x8000u ? 0xffffu : 0x8000u);
-    add_key(u << 16 | (0xffffu - (unsigned)c), c);
-  }
-  __device__ __forceinline__ float value(int j) const {
-    const unsigned k = key[j] >> 16;
-    const unsigned short h = (unsigned short)(k & 0x8000u ? k ^ 0x8000u : k ^ 0xffffu);
-    E z;
-    __builtin_memcpy(&z, &h, 2);
-    return (float)z;
-  }
-  __device__ __forceinline__ int cls(int j) const { return 0xffff - (int)(key[j] & 0xffffu); }
-};
-template <typename E, int K> struct BestOf { using type = Best16<E, K>; };
-template <int K> struct BestOf<float, K> { using type = Best<float, K>; };
 
-constexpr int PLANE_K = 32, PLANE_CLASSES = 65536;
+constexpr int PLANE_K = 32;
+template <typename E> constexpr int PLANE_CLASSES = CLASS_BITS<E> ? (int)CLASS_BITS<E> + 1 : 65536;
 
 // SPLIT = 4: a block's four waves share 64 * PV pixels and take a quarter of the classes each (images too small to fill the device).
 template <typename E, int PV, int K, int SPLIT>
 __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, const LogprobOut o, const long long i0, const int tiles) {
-  using B = typename BestOf<E, K>::type;
+  using B = Best<E, K>;
+  constexpr bool IDS = B::BITS == 0 && K > 0;
   constexpr int LANES = 256 / SPLIT, UN = 8;
   __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][3][PV][SPLIT > 1 ? 64 : 1];
   __shared__ unsigned lists[SPLIT > 1 ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
-  __shared__ int ids[SPLIT > 1 && sizeof(B) > 4 * (K > 0 ? K : 1) ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
+  __shared__ int ids[SPLIT > 1 && IDS ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 && IDS ? 64 : 1];
   const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, pl = threadIdx.x & (LANES - 1);
   const long long i = i0 + blockIdx.x / (unsigned)tiles;
   const long long first = (long long)(blockIdx.x % (unsigned)tiles) * (LANES * PV) + pl * PV;
@@ -522,15 +514,24 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   B best[PV];
 #pragma unroll
   for (int v = 0; v < PV; ++v) { m[v] = -INFINITY; s[v] = u[v] = 0.f; }
-  for (int c = c0; c < c1; c += UN) {
-    E q[UN][PV];
-    float x[UN][PV];
+  // The next classes are on their way while these are worked on: an image's waves are all resident at once, and without it they all wait
+  // for memory at the same time.
+  const auto load = [&](E(&q)[UN][PV], int c) {
 #pragma unroll
     for (int n = 0; n < UN; ++n) load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, q[n]);
+  };
+  const auto work = [&](const E(&q)[UN][PV], int c) {
+    float x[UN][PV];
 #pragma unroll
     for (int n = 0; n < UN; ++n)
 #pragma unroll
-      for (int v = 0; v < PV; ++v) x[n][v] = c + n < c1 ? (float)q[n][v] : -INFINITY;
+      for (int v = 0; v < PV; ++v) x[n][v] = (float)q[n][v];
+    if (c + UN > c1) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+#pragma unroll
+        for (int v = 0; v < PV; ++v) x[n][v] = c + n < c1 ? x[n][v] : -INFINITY;
+    }
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
       float nm = m[v];
@@ -551,9 +552,18 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
       for (int n = 0; n < UN; ++n)
         if (c + n < c1) {
 #pragma unroll
-          for (int v = 0; v < PV; ++v) best[v].add(q[n][v], c + n);
+          for (int v = 0; v < PV; ++v) best[v].add(x[n][v], c + n);
         }
     }
+  };
+  E qa[UN][PV], qb[UN][PV];
+  load(qa, c0);
+  for (int c = c0; c < c1; c += 2 * UN) {
+    if (c + UN < c1) load(qb, c + UN);
+    work(qa, c);
+    if (c + UN >= c1) break;
+    if (c + 2 * UN < c1) load(qa, c + 2 * UN);
+    work(qb, c + UN);
   }
   if constexpr (SPLIT > 1) {
     if (wv > 0) {
@@ -565,7 +575,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
 #pragma unroll
         for (int j = 0; j < K; ++j) {
           lists[wv - 1][j][v][pl] = best[v].key[j];
-          if constexpr (sizeof(B) > 4 * (K > 0 ? K : 1)) ids[wv - 1][j][v][pl] = best[v].cls(j);
+          if constexpr (IDS) ids[wv - 1][j][v][pl] = best[v].cls(j);
         }
       }
     }
@@ -585,7 +595,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
           for (int j = 0; j < K; ++j) {        // the other waves' classes are higher: equal keys stay behind
             const unsigned k = lists[w][j][v][pl];
             int id = 0;
-            if constexpr (sizeof(B) > 4 * (K > 0 ? K : 1)) id = ids[w][j][v][pl];
+            if constexpr (IDS) id = ids[w][j][v][pl];
             best[v].add_key(k, id);
           }
         }
@@ -593,21 +603,70 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
     }
   }
   if (first >= a.p) return;
+  const long long r = i * a.p + px.px, ot = i * o.tn + px.px * o.tp;
+  float base[PV], ls[PV], out[PV];
+  bool empty[PV], is_class[PV];
+  long long y[PV];
 #pragma unroll
   for (int v = 0; v < PV; ++v) {
-    if (!px.own(v)) continue;
-    const long long r = i * a.p + px.px + v;
-    const long long y = o.label ? o.label[r] : 0;
-    const bool empty = o.label && y == o.ignore, is_class = y >= 0 && y < a.C;
-    const float base = m[v] == -INFINITY ? 0.f : m[v], ls = log2_(s[v]) * LN2;
-    if (empty) void_row(o, r, a.R);
-    else finish_row(o, r, a, base, s[v], u[v], ls, is_class, o.logprob && is_class ? load1(z + y * a.sc + v) : 0.f);
-    const long long ot = i * o.tn + (px.px + v) * o.tp;
+    y[v] = o.label ? o.label[r + v] : 0;
+    empty[v] = o.label && y[v] == o.ignore;
+    is_class[v] = y[v] >= 0 && y[v] < a.C;
+    base[v] = m[v] == -INFINITY ? 0.f : m[v];
+    ls[v] = log2_(s[v]) * LN2;
+  }
+  if (o.logprob) {
 #pragma unroll
-    for (int j = 0; j < K; ++j)
-      if (j < o.k) {
-        o.top_ids[ot + j * o.tk] = empty ? -1 : best[v].cls(j);
-        o.top_lp[ot + j * o.tk] = empty || s[v] == 0.f ? -INFINITY : (best[v].value(j) - base) * a.invT - ls;
+    for (int v = 0; v < PV; ++v) {
+      const float zy = is_class[v] && !empty[v] ? load1(z + y[v] * a.sc + v) : 0.f;
+      out[v] = empty[v] ? 0.f : !is_class[v] ? NAN : s[v] == 0.f ? -INFINITY : (zy - base[v]) * a.invT - ls[v];
+    }
+    px.put(o.logprob + r, 1, out);
+  }
+  if (o.entropy) {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) out[v] = empty[v] || s[v] == 0.f ? 0.f : ls[v] - u[v] / s[v] * LN2;
+    px.put(o.entropy + r, 1, out);
+  }
+  if (o.lse) {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) out[v] = empty[v] ? 0.f : base[v] * a.invT + ls[v];
+    px.put(o.lse + r, 1, out);
+  }
+  if (o.stats) {
+#pragma unroll
+    for (int v = 0; v < PV; ++v) out[v] = empty[v] ? 0.f : base[v];
+    px.put(o.stats + r, 1, out);
+#pragma unroll
+    for (int v = 0; v < PV; ++v) out[v] = empty[v] ? 0.f : ls[v];
+    px.put(o.stats + a.R + r, 1, out);
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (j < o.k) {
+      int id[PV];
+#pragma unroll
+      for (int v = 0; v < PV; ++v) {
+        id[v] = empty[v] ? -1 : best[v].cls(j);
+        out[v] = empty[v] || s[v] == 0.f ? -INFINITY : (best[v].value(j) - base[v]) * a.invT - ls[v];
+      }
+      px.put(o.top_ids + ot + j * o.tk, o.tp, id);
+      px.put(o.top_lp + ot + j * o.tk, o.tp, out);
+    }
+  if (K > 0) {
+#pragma unroll
+    for (int v = 0; v < PV; ++v)
+      if (s[v] != s[v] && !empty[v] && px.own(v)) {      // a NaN or +inf: the alternatives once more
+        unsigned long long prev = ~0ull;
+        for (int j = 0; j < o.k; ++j) {
+          unsigned long long top = 0;
+          for (int c = 0; c < a.C; ++c) {
+            const unsigned long long key = pair_key(load1(z + c * a.sc + v), c);
+            top = key < prev && key > top ? key : top;
+          }
+          prev = top;
+          o.top_ids[ot + v * o.tp + j * o.tk] = (int)~(unsigned)top;
+        }
       }
   }
 }
@@ -626,7 +685,7 @@ struct RowGrad {
   float m, ls, A, B, G;
   long long y;
   bool dead;                 // void, or nothing but -inf: no gradient
-  __device__ __forceinline__ RowGrad(const Logits& a, const LogprobGrad& g, long long r) {
+  __device__ __forceinline__ void init(const Logits& a, const LogprobGrad& g, long long r) {
     y = g.label ? g.label[r] : -1;
     m = g.stats[r];
     ls = g.stats[a.R + r];
@@ -645,29 +704,34 @@ struct RowGrad {
 
 // Contiguous classes: G lanes to a row (8, 64) or a block to a segment of SEG chunks a lane; one read, one write, no reductions.
 template <typename E, int G>
-__global__ __launch_bounds__(256) void logprobs_bwd_rows_kernel(const Logits a, const LogprobGrad g, const int segs) {
+__global__ __launch_bounds__(256) void logprobs_bwd_rows_kernel(const Logits a, const LogprobGrad g) {
   constexpr int V = VEC<E>, SEG = 4;
   const int l = threadIdx.x % G;
-  const long long step = (long long)gridDim.x * (256 / G), items = a.R * segs;
-  for (long long it = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; it < items; it += step) {
-    long long r = it;
-    int seg = 0;
-    if (segs > 1) {
-      r = items <= 0x7fffffff ? (unsigned)it / (unsigned)segs : it / segs;
-      seg = (int)(it - r * segs);
-    }
-    const RowGrad f(a, g, r);
+  const int seg = blockIdx.x;              // G < 256: 0
+  const long long step = (long long)gridDim.y * (256 / G);
+  for (long long r = (long long)blockIdx.y * (256 / G) + threadIdx.x / G; r < a.R; r += step) {
+    RowGrad f;
+    f.init(a, g, r);
     const E* z = (const E*)a.z + a.at(r);
-    E* dz = (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp);
-    for (int q = 0; q < (G == 256 ? SEG : (a.C + G * V - 1) / (G * V)); ++q) {
-      const int c = (G == 256 ? seg * (SEG * G * V) : 0) + (q * G + l) * V;
-      if (c >= a.C) break;
-      float x[V], old[V];
-      const int b = load_chunk<G == 8>(z, c, a.C, x);
-      if (g.accumulate) load_chunk<G == 8>((const E*)dz, c, a.C, old);
+    E* dz = (E*)g.dz + row_at(a, r, g.dn, g.dp);
+    const int c1 = G == 256 ? min(a.C, (seg + 1) * (SEG * G * V)) : a.C;
+    for (int c0 = G == 256 ? seg * (SEG * G * V) : 0; c0 < c1; c0 += SEG * G * V) {
+      Vec<E> q[SEG], old[SEG];
+      int b[SEG];
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[e] = f(a, x[e], b + e) + (g.accumulate ? old[e] : 0.f);
-      store_chunk(dz, c, b, a.C, x);
+      for (int i = 0; i < SEG; ++i) {
+        b[i] = load_raw<G == 8>(z, c0 + (i * G + l) * V, a.C, q[i]);
+        if (g.accumulate) load_raw<G == 8>((const E*)dz, c0 + (i * G + l) * V, a.C, old[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < SEG; ++i) {
+        const int c = c0 + (i * G + l) * V;
+        if (c >= c1) break;
+        float x[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] = f(a, (float)q[i][e], b[i] + e) + (g.accumulate ? (float)old[i][e] : 0.f);
+        store_chunk(dz, c, b[i], a.C, x);
+      }
     }
   }
 }
@@ -683,7 +747,9 @@ __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a
   const Px<PV> px(first, a.p);
   const E* z = (const E*)a.z + i * a.sn + px.px;
   E* dz = (E*)g.dz + i * g.dn + px.px;
-  const RowGrad f0(a, g, i * a.p + px.px), f1(a, g, i * a.p + px.px + PV - 1);
+  RowGrad f[PV];
+#pragma unroll
+  for (int v = 0; v < PV; ++v) f[v].init(a, g, i * a.p + px.px + v);
   const int c0 = blockIdx.y * slice, c1 = min(a.C, c0 + slice);
   for (int c = c0; c < c1; c += UN) {
     E q[UN][PV], old[UN][PV];
@@ -696,7 +762,7 @@ __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a
     for (int n = 0; n < UN; ++n) {
       if (c + n >= c1) break;
 #pragma unroll
-      for (int v = 0; v < PV; ++v) q[n][v] = (E)((v ? f1 : f0)(a, (float)q[n][v], c + n) + (g.accumulate ? (float)old[n][v] : 0.f));
+      for (int v = 0; v < PV; ++v) q[n][v] = (E)(f[v](a, (float)q[n][v], c + n) + (g.accumulate ? (float)old[n][v] : 0.f));
       if (px.own(0)) {
         store_px<E, PV>(dz + (c + n) * g.dc, q[n]);
       } else {
@@ -742,7 +808,7 @@ template <typename E>
 void logprobs_bwd(const Logits& a, const LogprobGrad& g, hipStream_t stream) {
   if (a.C > 1 && a.sc != 1) {
     constexpr int PV = sizeof(E) == 2 ? 2 : 1;
-    const int pv = a.p > 1 ? PV : 1;
+    const int pv = a.p >= PV ? PV : 1;
     const long long tiles = (a.p + 256 * pv - 1) / (256 * pv);
     // slices of the classes until there are about eight blocks a compute unit, none shorter than 16 classes
     const long long blocks = a.R / a.p * tiles;
@@ -756,18 +822,15 @@ void logprobs_bwd(const Logits& a, const LogprobGrad& g, hipStream_t stream) {
     });
     return;
   }
-  if (a.C <= 256) logprobs_bwd_rows_kernel<E, 8><<<capped((a.R + 31) / 32, 16384), 256, 0, stream>>>(a, g, 1);
-  else if (a.C <= 4 * 64 * VEC<E>) logprobs_bwd_rows_kernel<E, 64><<<capped((a.R + 3) / 4, 16384), 256, 0, stream>>>(a, g, 1);
-  else {
-    const int segs = (a.C + 4 * 256 * VEC<E> - 1) / (4 * 256 * VEC<E>);
-    logprobs_bwd_rows_kernel<E, 256><<<capped(a.R * segs, 1 << 20), 256, 0, stream>>>(a, g, segs);
-  }
+  if (a.C <= 256) logprobs_bwd_rows_kernel<E, 8><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, g);
+  else if (a.C <= 4 * 64 * VEC<E>) logprobs_bwd_rows_kernel<E, 64><<<dim3(1, capped((a.R + 3) / 4, 65535)), 256, 0, stream>>>(a, g);
+  else logprobs_bwd_rows_kernel<E, 256><<<seg_grid(a.R, a.C, 4 * 256 * VEC<E>), 256, 0, stream>>>(a, g);
 }
 
 template <typename E>
 void logprobs_fwd(const Logits& a, const LogprobOut& o, int type, void* scratch, hipStream_t stream) {
   if (a.C > 1 && a.sc != 1) {
-    if (o.k > PLANE_K || a.C > PLANE_CLASSES) {
+    if (o.k > PLANE_K || a.C > PLANE_CLASSES<E>) {
       logprobs_fwd_kernel<E><<<row_blocks(a.R), 256, 0, stream>>>(a, o);
     } else {
       logprobs_planes<E>(a, o, stream);
@@ -782,16 +845,18 @@ void logprobs_fwd(const Logits& a, const LogprobOut& o, int type, void* scratch,
     if (o.k) logprobs_rows_kernel<E, G, NV, true><<<blocks, 256, 0, stream>>>(a, o);         \
     else logprobs_rows_kernel<E, G, NV, false><<<blocks, 256, 0, stream>>>(a, o);            \
   } while (0)
-    if (chunks <= 8) ROWS(8, 1);
-    else if (chunks <= 16) ROWS(8, 2);
-    else if (chunks <= 24) ROWS(8, 3);
-    else if (chunks <= 32) ROWS(8, 4);
-    else if (VEC<E> == 4 && chunks <= 40) ROWS(8, VEC<E> == 4 ? 5 : 1);
-    else if (VEC<E> == 4 && chunks <= 64) ROWS(8, VEC<E> == 4 ? 8 : 1);
+    constexpr bool W4 = VEC<E> == 4;
+    if (chunks <= 4) ROWS(4, 1);
+    else if (chunks <= 8) ROWS(4, 2);
+    else if (chunks <= 12) ROWS(4, 3);
+    else if (chunks <= 20) ROWS(4, 5);
+    else if (W4 && chunks <= 40) ROWS(4, W4 ? 10 : 1);
+    else if (!W4 && chunks <= 32) ROWS(8, W4 ? 1 : 4);
+    else if (W4 && chunks <= 64) ROWS(8, W4 ? 8 : 1);
     else if (chunks <= 64) ROWS(64, 1);
     else if (chunks <= 128) ROWS(64, 2);
     else if (chunks <= 256) ROWS(64, 4);
-    else ROWS(64, VEC<E> == 4 ? 8 : 1);
+    else ROWS(64, W4 ? 8 : 1);
 #undef ROWS
     return;
   }

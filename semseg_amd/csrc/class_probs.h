@@ -36,7 +36,7 @@ __device__ __forceinline__ unsigned long long pair_key(float z, int c) {
   return ((unsigned long long)order_key(z) << 32) | (unsigned)~c;
 }
 
-// ---- reductions over groups of G = 8 or 64 neighbouring lanes: data-parallel moves inside a row of 16 lanes, swaps of rows beyond
+// ---- reductions over groups of G = 4, 8 or 64 neighbouring lanes: data-parallel moves inside a row of 16 lanes, swaps of rows beyond
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) { return (unsigned)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true); }
 constexpr int XOR1 = 0xB1, XOR2 = 0x4E, HALF_MIRROR = 0x141, MIRROR = 0x140;
@@ -47,7 +47,7 @@ __device__ __forceinline__ T group_reduce(T v, F f) {
   const auto val = [](unsigned x) { return __builtin_bit_cast(T, x); };
   v = f(v, val(dpp<XOR1>(bits(v))));
   v = f(v, val(dpp<XOR2>(bits(v))));
-  v = f(v, val(dpp<HALF_MIRROR>(bits(v))));
+  if (G >= 8) v = f(v, val(dpp<HALF_MIRROR>(bits(v))));
   if (G == 64) {
     v = f(v, val(dpp<MIRROR>(bits(v))));
     // both operands v: the odd rows (the upper half) of the one and the even rows (the lower half) of the other change places
@@ -109,6 +109,42 @@ __device__ __forceinline__ int load_chunk(const E* z, int s, int C, float (&x)[V
   for (int e = 0; e < V; ++e) x[e] = s + e < C ? load1(z + s + e) : -INFINITY;
   return s;
 }
+// N chunks of a row, the i-th from class first + i * step on, into x[i]; returns their first classes in b.  All loads go out before the
+// first value is looked at (a branch for the cut chunk behind each load would make the loads wait for each other), chunks in the same
+// place for all lanes are masked only where the row can end in one of them.
+template <int N, bool SHORT, typename E>
+__device__ __forceinline__ void load_chunks(const E* z, int first, int step, int C, float (&x)[N][VEC<E>], int (&b)[N]) {
+  constexpr int V = VEC<E>;
+  if (SHORT && C < V) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) b[i] = load_chunk<true>(z, first + i * step, C, x[i]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    b[i] = min(first + i * step, C - V);
+    load_vec(z + b[i], x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (__any(first + i * step + V > C)) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[i][e] = b[i] + e >= first + i * step ? x[i][e] : -INFINITY;
+    }
+}
+// One chunk as it lies in memory (for a gradient: what it holds below class s is never stored), and its values
+template <bool SHORT, typename E>
+__device__ __forceinline__ int load_raw(const E* z, int s, int C, Vec<E>& q) {
+  constexpr int V = VEC<E>;
+  if (SHORT && C < V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = s + e < C ? z[s + e] : (E)0.f;
+    return s;
+  }
+  const int b = min(s, C - V);
+  q = __builtin_bit_cast(Vec<E>, reinterpret_cast<const Raw<E>*>(z + b)->v);
+  return b;
+}
 template <typename E>
 __device__ __forceinline__ void store_chunk(E* z, int s, int b, int C, const float (&x)[VEC<E>]) {
   if (s + VEC<E> <= C) {
@@ -128,23 +164,24 @@ __device__ __forceinline__ void zero_row(E* dz, int l, int C) {
   for (int c = l * VEC<E>; c < C; c += G * VEC<E>) store_chunk(dz, c, C < VEC<E> ? c : min(c, C - VEC<E>), C, x);
 }
 
-// i * s0 + j * s1 of row r = i * p + j; 64-bit divisions (~150 instructions) are kept out of the usual cases
-__device__ __forceinline__ long long row_at(long long r, long long p, long long R, long long s0, long long s1) {
-  if (p == R) return r * s1;
-  if (R <= 0x7fffffff) {
-    const unsigned i = (unsigned)r / (unsigned)p;
-    return i * s0 + ((unsigned)r - i * (unsigned)p) * s1;
-  }
-  return (r / p) * s0 + (r % p) * s1;
-}
-
 struct Logits {
   const void* z;
   long long R, p, sn, sp, sc;
   int C;
   float invT, scale2;      // 1 / T, log2(e) / T
-  __device__ __forceinline__ long long at(long long r) const { return row_at(r, p, R, sn, sp); }
+  double inv_p;            // 1 / p
+  __device__ __forceinline__ long long at(long long r) const;
 };
+// i * s0 + j * s1 of row r = i * p + j.  r < 2^40: the quotient by a multiplication in fp64 is off by one at most (an integer division
+// of 64 bits is ~150 instructions, and kernels of a few microseconds are short).
+__device__ __forceinline__ long long row_at(const Logits& a, long long r, long long s0, long long s1) {
+  if (a.p == a.R) return r * s1;
+  long long i = (long long)((double)r * a.inv_p), j = r - i * a.p;
+  if (j < 0) { --i; j += a.p; }
+  if (j >= a.p) { ++i; j -= a.p; }
+  return i * s0 + j * s1;
+}
+__device__ __forceinline__ long long Logits::at(long long r) const { return row_at(*this, r, sn, sp); }
 
 // s, u taken about `from` become sums about `to` >= from (u's terms carry a factor d); an empty sum may come from -inf
 __device__ __forceinline__ void rescale(float& s, float& u, float from, float to, float scale2) {
@@ -164,6 +201,10 @@ __device__ __forceinline__ void load_px(const E* p, E (&q)[PV]) {
     struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
     const u32x2 w = reinterpret_cast<const W*>(p)->v;
     __builtin_memcpy(q, &w, 8);
+  } else if constexpr (PV * sizeof(E) == 16) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x4 v; };
+    const u32x4 w = reinterpret_cast<const W*>(p)->v;
+    __builtin_memcpy(q, &w, 16);
   } else {
 #pragma unroll
     for (int v = 0; v < PV; ++v) q[v] = p[v];
@@ -181,6 +222,11 @@ __device__ __forceinline__ void store_px(E* p, const E (&q)[PV]) {
     u32x2 w;
     __builtin_memcpy(&w, q, 8);
     reinterpret_cast<W*>(p)->v = w;
+  } else if constexpr (PV * sizeof(E) == 16) {
+    struct __attribute__((packed, aligned(alignof(E)))) W { u32x4 v; };
+    u32x4 w;
+    __builtin_memcpy(&w, q, 16);
+    reinterpret_cast<W*>(p)->v = w;
   } else {
 #pragma unroll
     for (int v = 0; v < PV; ++v) p[v] = q[v];
@@ -193,6 +239,17 @@ struct Px {
   long long px, p0, P;
   __device__ __forceinline__ Px(long long first, long long P_) : px(first < P_ - PV ? first : P_ - PV), p0(first), P(P_) {}
   __device__ __forceinline__ bool own(int v) const { return px + v >= p0; }
+  // the own values of `x` to p, p + step, ...: together where they lie side by side
+  template <typename T>
+  __device__ __forceinline__ void put(T* p, long long step, const T (&x)[PV]) const {
+    if (step == 1 && own(0)) {
+      store_px<T, PV>(p, x);
+    } else {
+#pragma unroll
+      for (int v = 0; v < PV; ++v)
+        if (own(v)) p[v * step] = x[v];
+    }
+  }
 };
 
 // ---- host side
@@ -202,7 +259,7 @@ inline bool logits_ok(const void* z, int type, long long n, long long p, int C, 
 // rows: contiguous classes; planes: contiguous pixels (of fewer than 2^31 to an image)
 inline bool layout_ok(int C, long long p, long long sp, long long sc) { return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 31)); }
 inline Logits logits_of(const void* z, long long n, long long p, int C, long long sn, long long sp, long long sc, float T) {
-  return Logits{z, n * p, p, sn, sp, sc, C, 1.f / T, LOG2E / T};
+  return Logits{z, n * p, p, sn, sp, sc, C, 1.f / T, LOG2E / T, 1.0 / (double)p};
 }
 
 // Slices of a row of more classes than ROW_CLASSES: none with 512 rows or more (two blocks a compute unit), else about 1024 blocks in
@@ -220,6 +277,12 @@ inline Split split_rows(int type, long long R, int C) {
   return Split{(C + slice - 1) / slice, slice, (iters + 127) / 128};
 }
 inline int capped(long long blocks, int cap) { return (int)(blocks < cap ? blocks : cap); }
+
+// a block to every segment of a row, rows in a loop beyond what a grid holds
+inline dim3 seg_grid(long long R, int C, int seg) {
+  const int segs = (C + seg - 1) / seg, most = (1 << 23) / segs;
+  return dim3(segs, capped(R, most < 1 ? 1 : most > 65535 ? 65535 : most));
+}
 
 // launch(first image, images): groups of images whose grids stay below 2^32 lanes
 template <typename F>

@@ -31,29 +31,35 @@ struct RowTeacher {
   int id[NE];
   float q[NE], lq[NE], qsum, qrest;
   bool any, bad;             // any entry present; an id that is no class
+  // ids and values on their way, before anything else of the row is waited for
+  long long c_[NE];
   __device__ __forceinline__ RowTeacher(const Teacher& t, const Logits& a, long long r, int l) {
-    const long long io = row_at(r, a.p, a.R, t.in, t.ip), vo = row_at(r, a.p, a.R, t.vn, t.vp);
-    unsigned flags = 0;
-    float m = -INFINITY;
+    const long long io = row_at(a, r, t.in, t.ip), vo = row_at(a, r, t.vn, t.vp);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       const int j = i * TG + l;
-      id[i] = -1;
+      c_[i] = -1;
       lq[i] = -INFINITY;
       if (j < t.k) {
-        const long long c = t.id(io, j);
-        if (c >= a.C) flags |= 2u;
-        if (c >= 0 && c < a.C) {
-          flags |= 1u;
-          id[i] = (int)c;
-          lq[i] = t.value(vo, j);
-          m = fmaxf(m, lq[i]);
-        }
+        c_[i] = t.id(io, j);
+        lq[i] = t.value(vo, j);
       }
+    }
+  }
+  __device__ __forceinline__ void classes(const Logits& a) {
+    unsigned flags = 0;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      if (c_[i] >= a.C) flags |= 2u;
+      id[i] = c_[i] >= 0 && c_[i] < a.C ? (int)c_[i] : -1;
+      if (id[i] >= 0) flags |= 1u;
+      else lq[i] = -INFINITY;
     }
     flags = group_reduce<TG>(flags, [](unsigned x, unsigned y) { return x | y; });
     any = flags & 1u;
     bad = flags & 2u;
+  }
+  __device__ __forceinline__ void softmax(const Teacher& t, const Logits& a) {
     float s = 0.f;
     if (t.tail) {
 #pragma unroll
@@ -61,6 +67,9 @@ struct RowTeacher {
       qsum = group_sum<TG>(s);
       qrest = fmaxf(1.f - qsum, 0.f);
     } else {
+      float m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) m = fmaxf(m, lq[i]);
       m = group_max<TG>(m);
       if (m == -INFINITY) m = 0.f;
 #pragma unroll
@@ -158,28 +167,31 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(const double* part
 // The teacher's classes are few: a row is first written as if there were none, then the lanes that hold entries write theirs (from the
 // logits that they gather), behind the first stores in the same wave (or behind a barrier of the block).
 
-// Rows of at most 2048 contiguous classes: G lanes hold a row in registers.  GRAD: loss and gradient from one read of the logits.
+// Rows of at most 2048 contiguous classes: G lanes hold a row in registers (8 up to 256 classes; 4 lanes to a row save instructions, but
+// what bounds this kernel is the way from the entries' ids to the logits gathered there, and with them fewer waves share it: 57600 x 150,
+// k 8: 26.8 us, with 8 lanes 21).  GRAD: loss and gradient from one read of the logits.
 template <typename E, int G, int NV, int NE, bool GRAD, bool TAIL>
 __global__ __launch_bounds__(256) void distill_rows_kernel(const Logits a, const Teacher t, const DistillOut o, const DistillGrad g) {
   constexpr int V = VEC<E>;
-  constexpr bool SHORT = G == 8 && NV == 1;
+  constexpr bool SHORT = G < 64 && NV == 1;
   const int l = threadIdx.x % G;
   const long long step = (long long)gridDim.x * (256 / G);
   double loss = 0.0, wsum = 0.0;
   for (long long r = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; r < a.R; r += step) {
     const float w = t.weight ? t.weight[r] : 1.f;
-    E* dz = GRAD ? (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp) : nullptr;
+    E* dz = GRAD ? (E*)g.dz + row_at(a, r, g.dn, g.dp) : nullptr;
     bool dead = w == 0.f;
     if (!dead) {
       const E* z = (const E*)a.z + a.at(r);
+      RowTeacher<G, NE> q(t, a, r, l);
       float x[NV][V];
       int b[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) b[i] = load_chunk<SHORT>(z, (i * G + l) * V, a.C, x[i]);
-      const RowTeacher<G, NE> q(t, a, r, l);
+      load_chunks<NV, SHORT>(z, l * V, G * V, a.C, x, b);
+      q.classes(a);
       float zj[NE];
 #pragma unroll
       for (int i = 0; i < NE; ++i) zj[i] = q.id[i] >= 0 ? load1(z + q.id[i]) : -INFINITY;
+      q.softmax(t, a);
       float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -321,7 +333,7 @@ __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, con
   if (t.weight && t.weight[r] == 0.f) return;
   const E* z = (const E*)a.z + a.at(r);
   if (t.tail) {
-    const long long io = row_at(r, a.p, a.R, t.in, t.ip);
+    const long long io = row_at(a, r, t.in, t.ip);
     for (int j = tid; j < t.k; j += 256) {
       const long long c = t.id(io, j);
       ids[j] = c >= 0 && c < a.C ? (int)c : -1;
@@ -413,7 +425,9 @@ __global__ __launch_bounds__(256) void distill_join_kernel(const Logits a, const
       continue;
     }
     const E* z = (const E*)a.z + a.at(r);
-    const RowTeacher<64, 1> q(t, a, r, lane);
+    RowTeacher<64, 1> q(t, a, r, lane);
+    q.classes(a);
+    q.softmax(t, a);
     const float zj = q.id[0] >= 0 ? load1(z + q.id[0]) : -INFINITY;
     const float* part = d.part + (r * d.nsplit + (lane < d.nsplit ? lane : 0)) * 2;
     const float m1 = lane < d.nsplit ? part[0] : -INFINITY;
@@ -455,22 +469,19 @@ __global__ __launch_bounds__(256) void distill_join_kernel(const Logits a, const
 }
 
 // The gradient from the forward call's statistics: G lanes to a row (8, 64), or a block to a segment of SEG chunks a lane.
-template <typename E, int G>
-__global__ __launch_bounds__(256) void distill_bwd_rows_kernel(const Logits a, const Teacher t, const DistillGrad g, const int segs) {
-  constexpr int V = VEC<E>, SEG = 4, TG = G < 64 ? G : 64, NE = MAXK / TG;
+template <typename E, int G, int NE>
+__global__ __launch_bounds__(256) void distill_bwd_rows_kernel(const Logits a, const Teacher t, const DistillGrad g) {
+  constexpr int V = VEC<E>, SEG = 4, TG = G < 64 ? G : 64;
   const int l = threadIdx.x % G;
-  const long long step = (long long)gridDim.x * (256 / G), items = a.R * segs;
-  for (long long it = (long long)blockIdx.x * (256 / G) + threadIdx.x / G; it < items; it += step) {
-    long long r = it;
-    int seg = 0;
-    if (segs > 1) {
-      r = items <= 0x7fffffff ? (unsigned)it / (unsigned)segs : it / segs;
-      seg = (int)(it - r * segs);
-    }
+  const int seg = blockIdx.x;              // G < 256: 0
+  const long long step = (long long)gridDim.y * (256 / G);
+  for (long long r = (long long)blockIdx.y * (256 / G) + threadIdx.x / G; r < a.R; r += step) {
     const float w = t.weight ? t.weight[r] : 1.f, base = g.stats[r], ls = g.stats[a.R + r], lpt = g.stats[2 * a.R + r];
-    E* dz = (E*)g.dz + row_at(r, a.p, a.R, g.dn, g.dp);
+    E* dz = (E*)g.dz + row_at(a, r, g.dn, g.dp);
     const int c0 = G == 256 ? seg * (SEG * G * V) : 0, c1 = G == 256 ? min(a.C, c0 + SEG * G * V) : a.C;
-    const RowTeacher<TG, NE> q(t, a, r, threadIdx.x % TG);
+    RowTeacher<TG, NE> q(t, a, r, threadIdx.x % TG);
+    q.classes(a);
+    q.softmax(t, a);
     const bool dead = w == 0.f || q.bad || !q.any || ls == -INFINITY;
     const E* z = (const E*)a.z + a.at(r);
     const bool rest = t.tail && lpt != INFINITY;
@@ -491,21 +502,33 @@ __global__ __launch_bounds__(256) void distill_bwd_rows_kernel(const Logits a, c
       }
     }
     if (G == 256) __syncthreads();       // with accumulate: the entries' old values are read before the row is written
-    for (int c = c0 + l * V; c < c1; c += G * V) {
-      float x[V], old[V];
-      int b = c;
-      if (dead) {
-        if (g.accumulate) break;
+    if (dead) {
+      if (!g.accumulate) {
+        float x[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = 0.f;
-        if (c + V > a.C) b = G == 8 && a.C < V ? c : a.C - V;
-      } else {
-        b = load_chunk<G == 8>(z, c, a.C, x);
-        if (g.accumulate) load_chunk<G == 8>((const E*)dz, c, a.C, old);
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = f * exp2_(((x[e] - base) * a.invT - off) * LOG2E) + (g.accumulate ? old[e] : 0.f);
+        for (int c = c0 + l * V; c < c1; c += G * V) store_chunk(dz, c, G == 8 && a.C < V ? c : min(c, a.C - V), a.C, x);
       }
-      store_chunk(dz, c, b, a.C, x);
+    } else {
+      for (int cs = c0; cs < c1; cs += SEG * G * V) {
+        Vec<E> q[SEG], old[SEG];
+        int b[SEG];
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) {
+          b[i] = load_raw<G == 8>(z, cs + (i * G + l) * V, a.C, q[i]);
+          if (g.accumulate) load_raw<G == 8>((const E*)dz, cs + (i * G + l) * V, a.C, old[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < SEG; ++i) {
+          const int c = cs + (i * G + l) * V;
+          if (c >= c1) break;
+          float x[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            x[e] = f * exp2_(((float)q[i][e] - base) * a.scale2 - off * LOG2E) + (g.accumulate ? (float)old[i][e] : 0.f);
+          store_chunk(dz, c, b[i], a.C, x);
+        }
+      }
     }
     if (G == 256) {
       __syncthreads();
@@ -603,7 +626,7 @@ struct PixTeacher {
 // with SPLIT = 4 four waves share them and take a quarter of the classes each.
 template <typename E, int PV, int KR, int SPLIT, bool TAIL>
 __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits a, const Teacher t, const DistillOut o, const int tiles,
-                                                                    const long long all) {
+                                                                    const long long all, const double inv_tiles) {
   constexpr int COLS = 64 * PV;
   __shared__ float tiles_s[SPLIT][CH][COLS];
   __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][5][SPLIT > 1 ? COLS : 1];
@@ -613,7 +636,10 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
   const int c_lo = wv * per, c_hi = min(a.C, c_lo + per);
   double loss = 0.0, wsum = 0.0;
   for (long long it = blockIdx.x; it < all; it += gridDim.x) {
-    const long long i = all <= 0x7fffffff ? (unsigned)it / (unsigned)tiles : it / tiles, first = (it - i * tiles) * COLS + lane * PV;
+    long long i = (long long)((double)it * inv_tiles), at = it - i * tiles;      // as in row_at
+    if (at < 0) { --i; at += tiles; }
+    if (at >= tiles) { ++i; at -= tiles; }
+    const long long first = at * COLS + lane * PV;
     const Px<PV> px(first, a.p);
     const E* z = (const E*)a.z + i * a.sn + px.px;
     const long long r0 = i * a.p + px.px, io = i * t.in + px.px * t.ip, vo = i * t.vn + px.px * t.vp;
@@ -690,11 +716,10 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
       }
     }
     if (first >= a.p) continue;
+    float s0[PV], s1[PV], s2[PV], lr[PV];
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
-      if (!px.own(v)) continue;
-      const long long r = r0 + v;
-      const float w = t.weight ? t.weight[r] : 1.f;
+      const float w = t.weight ? t.weight[r0 + v] : 1.f;
       const float ls = log2_(s[v]) * LN2;
       float lpt = 0.f, kl = s[v] == 0.f ? (q[v].qsum > 0.f ? INFINITY : 0.f) : q[v].qlogq - (dot[v] * a.invT - q[v].qsum * ls);
       bool rest = TAIL;
@@ -719,15 +744,19 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
       if (!q[v].any) kl = 0.f;
       if (q[v].bad) kl = NAN;
       const bool on = w != 0.f;        // a masked row's logits have been read, but nothing of them goes on
-      o.stats[r] = on ? base[v] : 0.f;
-      o.stats[a.R + r] = on ? ls : 0.f;
-      o.stats[2 * a.R + r] = !on ? 0.f : TAIL && !rest ? INFINITY : lpt;
-      if (o.rows) o.rows[r] = on ? o.T2 * w * kl : 0.f;
-      if (on) {
+      s0[v] = on ? base[v] : 0.f;
+      s1[v] = on ? ls : 0.f;
+      s2[v] = !on ? 0.f : TAIL && !rest ? INFINITY : lpt;
+      lr[v] = on ? o.T2 * w * kl : 0.f;
+      if (on && px.own(v)) {
         loss += (double)w * (double)kl;
         wsum += (double)w;
       }
     }
+    px.put(o.stats + r0, 1, s0);
+    px.put(o.stats + a.R + r0, 1, s1);
+    px.put(o.stats + 2 * a.R + r0, 1, s2);
+    if (o.rows) px.put(o.rows + r0, 1, lr);
   }
   block_part<64 * SPLIT>(o.part, loss, wsum);
 }
@@ -820,24 +849,25 @@ int distill_blocks(const Logits& a, long long* all, int* split) {
   }
   *all = a.R;
   *split = 1;
-  return capped((a.R + (a.C <= 256 ? 31 : 3)) / (a.C <= 256 ? 32 : 4), PARTS);
+  const int rows = a.C > 256 ? 4 : 32;      // of a block: distill_rows_t's choice of lanes to a row
+  return capped((a.R + rows - 1) / rows, PARTS);
 }
 
 template <typename E, bool GRAD, bool TAIL>
 void distill_rows_t(const Logits& a, const Teacher& t, const DistillOut& o, const DistillGrad& g, int blocks, hipStream_t stream) {
   const int chunks = (a.C + VEC<E> - 1) / VEC<E>;
 #define DROWS(G, NV, NE) distill_rows_kernel<E, G, NV, NE, GRAD, TAIL><<<blocks, 256, 0, stream>>>(a, t, o, g)
+  constexpr bool W4 = VEC<E> == 4;
 #define DROWS8(NV) do { if (t.k <= 8) DROWS(8, NV, 1); else DROWS(8, NV, 8); } while (0)
   if (chunks <= 8) DROWS8(1);
   else if (chunks <= 16) DROWS8(2);
-  else if (chunks <= 32 && VEC<E> == 8) DROWS8(4);
   else if (chunks <= 24) DROWS8(3);
-  else if (chunks <= 40 && VEC<E> == 4) DROWS8(VEC<E> == 4 ? 5 : 1);
-  else if (chunks <= 64 && VEC<E> == 4) DROWS8(VEC<E> == 4 ? 8 : 1);
+  else if (W4 && chunks <= 40) DROWS8(W4 ? 5 : 1);
+  else if (chunks <= (W4 ? 64 : 32)) DROWS8(W4 ? 8 : 4);
   else if (chunks <= 64) DROWS(64, 1, 1);
   else if (chunks <= 128) DROWS(64, 2, 1);
   else if (chunks <= 256) DROWS(64, 4, 1);
-  else DROWS(64, VEC<E> == 4 ? 8 : 1, 1);
+  else DROWS(64, W4 ? 8 : 1, 1);
 #undef DROWS8
 #undef DROWS
 }
@@ -855,13 +885,13 @@ void distill_fwd(const Logits& a, const Teacher& t, const DistillOut& o, int typ
   const int blocks = distill_blocks<E>(a, &all, &split);
   if (a.C > 1 && a.sc != 1) {
     constexpr int PV = sizeof(E) == 2 ? 2 : 1;
-    const int pv = a.p > 1 ? PV : 1, tiles = (int)((a.p + 64 * pv - 1) / (64 * pv));
+    const int pv = a.p >= PV ? PV : 1, tiles = (int)((a.p + 64 * pv - 1) / (64 * pv));
 #define DPLANES(PV_, KR, SP)                                                                                              \
   do {                                                                                                                    \
-    if (t.tail) distill_planes_kernel<E, PV_, KR, SP, true><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all);         \
-    else distill_planes_kernel<E, PV_, KR, SP, false><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all);               \
+    if (t.tail) distill_planes_kernel<E, PV_, KR, SP, true><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all, 1.0 / tiles);         \
+    else distill_planes_kernel<E, PV_, KR, SP, false><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all, 1.0 / tiles);               \
   } while (0)
-    if (PV == 2 && pv == 1) DPLANES(1, 0, 4);
+    if (PV > 1 && pv == 1) DPLANES(1, 0, 4);
     else if (split == 1 && t.k <= 4) DPLANES(PV, 4, 1);
     else if (split == 1 && t.k <= 8) DPLANES(PV, 8, 1);
     else if (split == 1) DPLANES(PV, 0, 1);
@@ -886,8 +916,9 @@ void distill_fwd(const Logits& a, const Teacher& t, const DistillOut& o, int typ
 template <typename E>
 void distill_bwd(const Logits& a, const Teacher& t, const DistillGrad& g, hipStream_t stream) {
   if (a.C > 1 && a.sc != 1) {
-    constexpr int PV = sizeof(E) == 2 ? 2 : 1;
-    const int pv = a.p > 1 ? PV : 1;
+    // two pixels to a lane: 8 bytes a load and store of fp32 (4 x 150 x 473 x 473: 264 us, with one 290, with four 259 but slower on small images)
+    constexpr int PV = 2;
+    const int pv = a.p >= PV ? PV : 1;
     const long long tiles = (a.p + 64 * pv - 1) / (64 * pv), blocks = a.R / a.p * tiles;
     // slices of the classes until there are about 16 waves a compute unit
     const int tc = (a.C + CH - 1) / CH, slices = blocks >= 4096 ? 1 : (int)(4096 / blocks < tc ? 4096 / blocks : tc);
@@ -907,12 +938,10 @@ void distill_bwd(const Logits& a, const Teacher& t, const DistillGrad& g, hipStr
     });
     return;
   }
-  if (a.C <= 256) distill_bwd_rows_kernel<E, 8><<<capped((a.R + 31) / 32, 16384), 256, 0, stream>>>(a, t, g, 1);
-  else if (a.C <= 4 * 64 * VEC<E>) distill_bwd_rows_kernel<E, 64><<<capped((a.R + 3) / 4, 16384), 256, 0, stream>>>(a, t, g, 1);
-  else {
-    const int segs = (a.C + 4 * 256 * VEC<E> - 1) / (4 * 256 * VEC<E>);
-    distill_bwd_rows_kernel<E, 256><<<capped(a.R * segs, 1 << 20), 256, 0, stream>>>(a, t, g, segs);
-  }
+  if (a.C <= 256 && t.k <= 8) distill_bwd_rows_kernel<E, 8, 1><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, t, g);
+  else if (a.C <= 256) distill_bwd_rows_kernel<E, 8, 8><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, t, g);
+  else if (a.C <= 4 * 64 * VEC<E>) distill_bwd_rows_kernel<E, 64, 1><<<dim3(1, capped((a.R + 3) / 4, 65535)), 256, 0, stream>>>(a, t, g);
+  else distill_bwd_rows_kernel<E, 256, 1><<<seg_grid(a.R, a.C, 4 * 256 * VEC<E>), 256, 0, stream>>>(a, t, g);
 }
 
 // Scratch of a distillation call: partial sums, then the slices' maxima and sums of long rows
