@@ -500,8 +500,12 @@ template <typename E, int PV, int K, int SPLIT>
 __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, const LogprobOut o, const long long i0, const int tiles) {
   using B = Best<E, K>;
   constexpr bool IDS = B::BITS == 0 && K > 0;
+  // The label's logit is kept as it comes by (fp32), or fetched afterwards (16 bits): the one costs two instructions a logit, the other a
+  // memory line a pixel.  8 x 150 x 473 x 473 fp32: 250 against 265 us; 2 x 19 x 713 x 713 bf16, whose two pixels to a lane leave no
+  // instructions to spare: 24 against 21.
+  constexpr bool ZY = sizeof(E) == 4;
   constexpr int LANES = 256 / SPLIT, UN = 8;
-  __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][3][PV][SPLIT > 1 ? 64 : 1];
+  __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][4][PV][SPLIT > 1 ? 64 : 1];
   __shared__ unsigned lists[SPLIT > 1 ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
   __shared__ int ids[SPLIT > 1 && IDS ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 && IDS ? 64 : 1];
   const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, pl = threadIdx.x & (LANES - 1);
@@ -510,10 +514,18 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   const Px<PV> px(first, a.p);
   const E* z = (const E*)a.z + i * a.sn + px.px;
   const int per = (a.C + SPLIT - 1) / SPLIT, c0 = wv * per, c1 = min(a.C, c0 + per);
-  float m[PV], s[PV], u[PV];
+  float m[PV], s[PV], u[PV], zy[PV];
+  int yc[PV];
   B best[PV];
 #pragma unroll
-  for (int v = 0; v < PV; ++v) { m[v] = -INFINITY; s[v] = u[v] = 0.f; }
+  for (int v = 0; v < PV; ++v) {
+    m[v] = -INFINITY;
+    s[v] = u[v] = zy[v] = 0.f;
+    if (ZY) {
+      const long long y = o.logprob ? o.label[i * a.p + px.px + v] : -1;
+      yc[v] = y >= 0 && y < a.C ? (int)y : -1;
+    }
+  }
   // The next classes are on their way while these are worked on: an image's waves are all resident at once, and without it they all wait
   // for memory at the same time.
   const auto load = [&](E(&q)[UN][PV], int c) {
@@ -547,6 +559,12 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
         u[v] += w * fmaxf(d, -300.f);
       }
     }
+    if (ZY) {
+#pragma unroll
+      for (int n = 0; n < UN; ++n)
+#pragma unroll
+        for (int v = 0; v < PV; ++v) zy[v] = yc[v] == c + n ? x[n][v] : zy[v];
+    }
     if (K > 0) {
 #pragma unroll
       for (int n = 0; n < UN; ++n)
@@ -572,6 +590,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
         red[wv - 1][0][v][pl] = m[v];
         red[wv - 1][1][v][pl] = s[v];
         red[wv - 1][2][v][pl] = u[v];
+        if (ZY) red[wv - 1][3][v][pl] = zy[v];
 #pragma unroll
         for (int j = 0; j < K; ++j) {
           lists[wv - 1][j][v][pl] = best[v].key[j];
@@ -591,6 +610,8 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
         s[v] += os;
         u[v] += ou;
         m[v] = nm;
+        const int lo = (w + 1) * per;
+        if (ZY) zy[v] = yc[v] >= lo && yc[v] < min(a.C, lo + per) ? red[w][3][v][pl] : zy[v];
         if (K > 0) {
           for (int j = 0; j < K; ++j) {        // the other waves' classes are higher: equal keys stay behind
             const unsigned k = lists[w][j][v][pl];
@@ -618,8 +639,8 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   if (o.logprob) {
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
-      const float zy = is_class[v] && !empty[v] ? load1(z + y[v] * a.sc + v) : 0.f;
-      out[v] = empty[v] ? 0.f : !is_class[v] ? NAN : s[v] == 0.f ? -INFINITY : (zy - base[v]) * a.invT - ls[v];
+      if (!ZY) zy[v] = is_class[v] && !empty[v] ? load1(z + y[v] * a.sc + v) : 0.f;
+      out[v] = empty[v] ? 0.f : !is_class[v] ? NAN : s[v] == 0.f ? -INFINITY : (zy[v] - base[v]) * a.invT - ls[v];
     }
     px.put(o.logprob + r, 1, out);
   }
