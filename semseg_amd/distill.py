@@ -54,7 +54,7 @@ def _groups(sizes, strides):
     return out
 
 
-class _Geom:
+class Geom:
     """Rows of a logits tensor: (n, p, C), element strides and the number of row dimensions that make up n."""
 
     def __init__(self, z, dim):
@@ -104,16 +104,16 @@ def _check_logits(z, class_dim, temperature):
         raise ValueError("logits of shape %s hold no value" % (tuple(z.shape),))
     if not 0 < temperature < 3e38:
         raise ValueError("temperature must be positive and finite, got %r" % (temperature,))
-    return _Geom(z, dim)
+    return Geom(z, dim)
 
 
-def _check_rows(t, what, g, dtype, z):
+def _check_rows(t, what, g, dtype, device):
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError("%s must be a %s tensor" % (what, dtype))
     if tuple(t.shape) != g.shape:
         raise ValueError("%s has shape %s, the logits' rows %s" % (what, tuple(t.shape), g.shape))
-    if t.device != z.device:
-        raise ValueError("%s is on %s, the logits on %s" % (what, t.device, z.device))
+    if t.device != device:
+        raise ValueError("%s is on %s, the logits on %s" % (what, t.device, device))
 
 
 def _overlap(a, b):
@@ -184,7 +184,7 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255
     A row of -inf logits has log probabilities -inf, entropy 0 and no gradient."""
     g = _check_logits(logits, class_dim, temperature)
     if label is not None:
-        _check_rows(label, "label", g, torch.int64, logits)
+        _check_rows(label, "label", g, torch.int64, logits.device)
         label = label.contiguous()
     if isinstance(topk, bool) or not isinstance(topk, int) or not 0 <= topk <= min(TOP_MAX, g.C):
         raise ValueError("topk must be a whole number of [0, min(%d, classes = %d)], got %r" % (TOP_MAX, g.C, topk))
@@ -198,40 +198,45 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255
 # ---------------------------------------------------------------------------------------------
 # distillation
 # ---------------------------------------------------------------------------------------------
-def _check_teacher(logits, top_ids, top_values, temperature, weight, class_dim, reduction, reductions):
-    g = _check_logits(logits, class_dim, temperature)
+def _check_top(g, device, top_ids, top_values, weight):
+    """The teacher's entries of rows `g` on `device`, as the kernels take them."""
     if not isinstance(top_ids, torch.Tensor) or top_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError("top_ids must be an int32 or int64 tensor")
     if not isinstance(top_values, torch.Tensor) or top_values.dtype not in ops.TYPES:
         raise TypeError("top_logits must be an fp32, bf16 or fp16 tensor")
-    k = top_ids.shape[g.dim] if top_ids.dim() == logits.dim() else -1
+    k = top_ids.shape[g.dim] if top_ids.dim() == len(g.shape) + 1 else -1
     want = g.shape[:g.dim] + (k,) + g.shape[g.dim:]
     if k < 1 or tuple(top_ids.shape) != want or tuple(top_values.shape) != want:
         raise ValueError("top_ids %s and top_logits %s must have the logits' shape %s with the teacher's entries in the place of the "
-                         "classes" % (tuple(top_ids.shape), tuple(top_values.shape), tuple(logits.shape)))
+                         "classes" % (tuple(top_ids.shape), tuple(top_values.shape), g.shape[:g.dim] + (g.C,) + g.shape[g.dim:]))
     if k > TOP_MAX:
         raise ValueError("at most %d entries a row, got %d" % (TOP_MAX, k))
-    if top_ids.device != logits.device or top_values.device != logits.device:
-        raise ValueError("top_ids and top_logits must be on the logits' device %s" % (logits.device,))
+    if top_ids.device != device or top_values.device != device:
+        raise ValueError("top_ids and top_logits must be on the logits' device %s" % (device,))
     if top_values.requires_grad and torch.is_grad_enabled():
         raise ValueError("no gradient flows into the teacher: detach top_logits")
     if weight is not None:
-        _check_rows(weight, "weight", g, torch.float32, logits)
+        _check_rows(weight, "weight", g, torch.float32, device)
         if weight.requires_grad and torch.is_grad_enabled():
             raise ValueError("no gradient flows into the weights: detach them")
         weight = weight.contiguous()
-    if reduction not in reductions:
-        raise ValueError("reduction must be one of %s, got %r" % (", ".join(reductions), reduction))
-    _on_gpu(logits)
     out = []
     for t in (top_ids, top_values):
         s = g.strides_of(t)
         if s is None:
             t = t.contiguous()
             s = g.strides_of(t)
-        out.append((t, s))
-    (ids, ids_s), (top, top_s) = out
-    return g, (ids, ids_s, top, top_s, k, weight)
+        out += [t, s]
+    return (*out, k, weight)
+
+
+def _check_distill(logits, top_ids, top_values, temperature, weight, class_dim, reduction, reductions):
+    g = _check_logits(logits, class_dim, temperature)
+    teacher = _check_top(g, logits.device, top_ids, top_values, weight)
+    if reduction not in reductions:
+        raise ValueError("reduction must be one of %s, got %r" % (", ".join(reductions), reduction))
+    _on_gpu(logits)
+    return g, teacher
 
 
 def _distill(z, g, teacher, temperature, tail, reduction):
@@ -279,7 +284,7 @@ def distill_loss(logits, top_ids, top_logits, temperature=1.0, tail=False, weigh
     temperature=temperature)); what they leave of 1 is one more class, against the student's mass outside the entries.
     A negative id is an absent entry, a row without entries counts with loss 0; an id that is no class makes the loss NaN.
     weight: fp32 per row; rows of weight 0 are not read.  reduction: "mean" (over the weights' sum; NaN where that is 0), "sum", "none"."""
-    g, teacher = _check_teacher(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum", "none"))
+    g, teacher = _check_distill(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum", "none"))
     if logits.requires_grad and torch.is_grad_enabled():
         return _Distill.apply(logits, g, teacher, float(temperature), bool(tail), reduction)
     with _on_device(logits):
@@ -291,7 +296,7 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
     """(loss, grad_scale * gradient of the loss) in one call, outside autograd: what a training step that writes its own gradients uses.
     out: the tensor the gradient is written to (logits' shape and type; classes or pixels contiguous as in the logits), added to with
     accumulate=True; the default is a new one.  The loss itself is not scaled."""
-    g, teacher = _check_teacher(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum"))
+    g, teacher = _check_distill(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum"))
     dev = logits.device
     if out is None:
         if accumulate:

@@ -18,6 +18,7 @@ import torch.distributed as dist
 from torch import nn
 
 from . import ops
+from .distill import Geom
 from ._lib import debug
 
 F32 = torch.float32
@@ -376,6 +377,12 @@ class Engine:
         self._plan_gen = -1        # ARENA_GEN at record time
         self._plan_tries = 0
         self._plan_off = False     # three recordings failed: the engine stays on the launch-by-launch path
+        # a teacher's top classes of the main score map for the next backward (Trainer.step(..., top=...)): (ids, their strides, values,
+        # their strides, k, weight or None), temperature, tail, factor of the loss; what the distillation writes; Trainer's state
+        self.teacher = None
+        self._distill_bufs = None
+        self._teacher_sig = None
+        self._plan_top = None
         self.tape_hook = None  # callable(TapeOp) that must call op.fn(); set by tests only
         self._groups = {}
         self.syncbn_collectives_per_step = 0   # SyncBN all-reduces issued by the last forward + backward
@@ -1296,7 +1303,32 @@ class Engine:
                         s.N, s.H, s.W, rec["H"], rec["W"], s.C, rec["ignore"], scratch=self.scratch())
         s.ginit = True
 
+    def distill_buffers(self):
+        """What the distillation on the main scores writes beside their gradient; allocated before a step that uses it is recorded."""
+        if self._distill_bufs is None:
+            C = self.model.cls[4].weight.shape[0]
+            h, w = self.score_hw()
+            new = lambda n, dt: torch.empty(n, dtype=dt, device=self.device)  # noqa: E731
+            self._distill_bufs = dict(loss=new(1, F32), acc=new(2, F64), stats=new(3 * self.N * h * w, F32),
+                                      scratch=new(ops.distill_scratch_bytes(F32, 1, self.N * h * w, C, 1), torch.uint8))
+        return self._distill_bufs
+
+    def distill_bwd(self):
+        """Distillation from the teacher's top classes on the main scores, loss and gradient in one pass over them: d scores +=
+        factor * d(T^2 KL(teacher || scores)) / d scores, behind the cross entropy's, which writes that buffer."""
+        (ids, ids_s, top, top_s, k, weight), temperature, tail, factor = self.teacher
+        s = self._rec_main["scores"]
+        g = self.grad_of(s)
+        assert s.ginit
+        rows = Geom(s.data[..., :s.C].movedim(-1, 1), 1)
+        b = self.distill_buffers()
+        ops.distill_fwd_bwd(s.data, rows.geom, rows.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, "mean", b["stats"],
+                            b["acc"], b["loss"], factor, g, rows.strides, True, b["scratch"])
+
     # ------------------------------------------------------------------ whole-network passes
+    def score_hw(self):
+        return (self.H - 1) // 8 + 1, (self.W - 1) // 8 + 1
+
     def out_hw(self):
         z = self.model.zoom_factor
         return int((self.H - 1) / 8 * z + 1), int((self.W - 1) / 8 * z + 1)
@@ -1345,12 +1377,16 @@ class Engine:
             feat = psa_forward(self, a, cat) if m.use_psa else a
         return x_tmp, feat
 
-    def forward_eval(self, x):
+    def scores_eval(self, x):
+        """The main head's score map (Act, valid until the engine's next pass)."""
         # validation is a natural checkpoint for the label counts of the training steps before it (no pending copy: free)
         self._label_watch().poll(self.model.cls[4].weight.shape[0], wait=True)
         x = self._begin(x)
         x_tmp, feat = self._features(x)
-        scores = self.head(feat, self.model.cls, "m")
+        return self.head(feat, self.model.cls, "m")
+
+    def forward_eval(self, x):
+        scores = self.scores_eval(x)
         h, w = self.out_hw()
         ncls = scores.C
         if self.model.zoom_factor != 1:
@@ -1404,6 +1440,8 @@ class Engine:
         self._main = torch.cuda.current_stream()
         self._run(TapeOp("ce", lambda: self.ce_bwd(self._rec_main, gmain), dict(rec=self._rec_main, gloss=gmain, gmul=1.0)))
         self._run(TapeOp("ce", lambda: self.ce_bwd(self._rec_aux, gaux), dict(rec=self._rec_aux, gloss=gaux, gmul=1.0)))
+        if self.teacher is not None:
+            self._run(TapeOp("distill", self.distill_bwd, dict(rec=self._rec_main, teacher=self.teacher)))
         for op in reversed(self.tape):
             self._run(op)
         if self._side_used:

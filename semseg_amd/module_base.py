@@ -9,6 +9,7 @@ so `loss.backward()`, torch.optim.SGD, DistributedDataParallel and checkpointing
 import torch
 from torch import nn
 
+from .distill import class_logprobs
 from .engine import Engine
 
 
@@ -79,6 +80,22 @@ class HipSegModule(nn.Module):
                                                       or getattr(crit, "label_smoothing", 0.0) != 0.0):
             raise NotImplementedError("only CrossEntropyLoss(ignore_index=..., reduction='mean')")
         return ii
+
+    def top_logits(self, x, k, temperature=1.0):
+        """A teacher's answer to distil from: the k best classes of every point of the score map ([N, (h - 1) / 8 + 1, (w - 1) / 8 + 1],
+        before the upsampling) with their log probabilities, and the map's entropy and log-sum-exp (semseg_amd.distill.ClassLogprobs;
+        top_ids and top_logprobs are [N, k, h', w']).  Eval mode only; the tensors are new ones.  Hand (top_ids, top_logprobs) to
+        Trainer.step(..., top=...) or semseg_amd.distill.distill_loss."""
+        if self.training:
+            raise RuntimeError("top_logits answers as a teacher: put the model in eval mode")
+        assert x.dim() == 4 and (x.size(2) - 1) % 8 == 0 and (x.size(3) - 1) % 8 == 0
+        if not x.is_cuda:
+            raise RuntimeError("semseg_amd runs on the MI355X only: move the model and input to cuda "
+                               "(there is no CPU fallback)")
+        eng = self._engine(x, False)
+        with torch.no_grad():
+            s = eng.scores_eval(x.float())
+            return class_logprobs(s.data[..., :s.C].movedim(-1, 1), topk=k, temperature=temperature)
 
     def forward(self, x, y=None):
         x_size = x.size()

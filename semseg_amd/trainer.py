@@ -17,6 +17,7 @@ import torch.distributed as dist
 from . import engine as _engine
 from . import ops
 from ._lib import lib
+from .distill import Geom, _check_top
 from .engine import Engine
 from ._lib import debug
 from .plan import PlanError, StepPlan
@@ -34,11 +35,14 @@ def poly_learning_rate(base_lr, curr_iter, max_iter, power=0.9):
 
 class Trainer:
     def __init__(self, model, base_lr=0.01, momentum=0.9, weight_decay=1e-4, aux_weight=0.4,
-                 ignore_index=255, bucket_mb=32, sync_bn=True):
+                 ignore_index=255, bucket_mb=32, sync_bn=True, distill_weight=1.0, distill_temperature=1.0, distill_tail=False):
+        """distill_*: of the distillation in steps that are given a teacher's top classes (step's `top`): its weight beside the main loss,
+        and semseg_amd.distill.distill_loss's temperature and tail."""
         self.model = model
         self.base_lr, self.momentum, self.wd = base_lr, momentum, weight_decay
         self.aux_weight = aux_weight
         self.ignore_index = ignore_index
+        self.distill_weight, self.distill_temperature, self.distill_tail = distill_weight, distill_temperature, distill_tail
         self.device = next(model.parameters()).device
         self.world = dist.get_world_size() if (dist.is_available() and dist.is_initialized()) else 1
         self.dist_on = self.world > 1 or (os.environ.get("SEMSEG_FORCE_DIST") == "1" and dist.is_initialized())
@@ -126,8 +130,30 @@ class Trainer:
                 e.host_op(lambda view=view: e._works.append(dist.all_reduce(view, group=self.grad_group, async_op=True)))
 
     # ------------------------------------------------------------------ one optimisation step
-    def step(self, x, y, lr=None):
-        """x [N,3,H,W] fp32 cuda, y [N,h,w] int64 cuda (per-rank shard).  Returns (pred, main, aux)."""
+    def _set_teacher(self, e, top):
+        """The engine's teacher for this step; everything about it is checked before any work is launched."""
+        sig = None
+        if top is None:
+            e.teacher = None
+        else:
+            ids, values, weight = top if len(top) == 3 else (*top, None)
+            h, w = e.score_hw()
+            C = self.model.cls[4].weight.shape[0]
+            rows = Geom(torch.empty(e.N, h, w, C, device="meta").movedim(-1, 1), 1)
+            e.teacher = (_check_top(rows, e.device, ids, values, weight), float(self.distill_temperature), bool(self.distill_tail),
+                         float(self.distill_weight))
+            if not 0 < e.teacher[1] < 3e38:
+                raise ValueError("distill_temperature must be positive and finite, got %r" % (self.distill_temperature,))
+            sig = (tuple(ids.shape), ids.dtype, values.dtype, weight is None) + e.teacher[1:]
+            e.distill_buffers()
+        if sig != e._teacher_sig:         # what a recorded step bakes in of it (_host_signature)
+            e._teacher_sig, e._plan_candidate, e._plan_top = sig, None, None
+
+    def step(self, x, y, lr=None, top=None):
+        """x [N,3,H,W] fp32 cuda, y [N,h,w] int64 cuda (per-rank shard).  Returns (pred, main, aux).
+
+        top: a teacher's top classes of the score map, (ids, values) or (ids, values, weight) as distill_loss takes them ([N,k,h',w'];
+        HipSegModule.top_logits): adds distill_weight * distillation to the loss, and its value (unweighted) to what is returned."""
         lr = self.base_lr if lr is None else lr
         # the parameters must still be views of flat_w (model.to()/half()/load_state_dict(assign=True) break that
         # silently: SGD would then update a buffer nobody reads)
@@ -138,6 +164,7 @@ class Trainer:
         e = self.engine(x)
         if e.params_stale():
             raise RuntimeError("the module tree changed after the Trainer built its engine; build a new Trainer")
+        self._set_teacher(e, top)
         if not (self.use_plan and e.ktimer is None and e.tape_hook is None and not e._plan_off):
             if e._plan_replays:
                 self._set_step_state(e, lr, 0)      # the device part of the dropout counter belongs to replayed steps only
@@ -161,6 +188,8 @@ class Trainer:
         reference returns (model/pspnet.py:101-103, `losses.append(main_loss)`); `pred` IS the engine's buffer — valid until
         the next step of this engine, `.clone()` to keep ("Output lifetime")."""
         l = e._losses.clone()
+        if e.teacher is not None:
+            return out[0], l[0:1], l[1:2], e.distill_buffers()["loss"].clone()
         return out[0], l[0:1], l[1:2]
 
     def _step_eager(self, e, x, y, lr, lr_dev=None):
@@ -223,7 +252,7 @@ class Trainer:
         mods = tuple((m.training, getattr(m, "p", None), getattr(m, "momentum", None), getattr(m, "eps", None))
                      for m in e._sig_mods)
         return (mods, self.momentum, self.wd, self.ignore_index, self.aux_weight, self.world, self.g_main.data_ptr(),
-                self.g_aux.data_ptr())
+                self.g_aux.data_ptr(), e._teacher_sig)
 
     def _step_planned(self, e, x, y, lr, st):
         plan = e._plan
@@ -247,6 +276,7 @@ class Trainer:
                                                  e._plan_y.data_ptr(), ys.data_ptr(), ys.numel() * ys.element_size(),
                                                  self._step_state.data_ptr(), float(lr), float(lr) * 10.0,
                                                  e.drop_dev.data_ptr(), int(drop_off), ops._stream()), "step_begin")
+            self._plan_teacher(e)
             e._drop_calls += e._plan_drops
             if self.dist_on:
                 e._works = []
@@ -266,6 +296,24 @@ class Trainer:
             return self._step_eager(e, x, y, lr)
         return self._record(e, x, y, lr, st)
 
+    @staticmethod
+    def _plan_teacher(e):
+        """The teacher's entries into the buffers that a recorded step reads."""
+        if e.teacher is None:
+            return
+        (ids, _, values, _, k, weight), *how = e.teacher
+        if e._plan_top is None:
+            rows = Geom(torch.empty(e.N, *e.score_hw(), 2, device="meta").movedim(-1, 1), 1)
+            new = [rows.empty(k, t.dtype, e.device) for t in (ids, values)]
+            s = rows.strides_of(new[0])
+            e._plan_top = (new[0], s, new[1], s, k, None if weight is None else torch.empty_like(weight))
+        t = e._plan_top
+        t[0].copy_(ids)
+        t[2].copy_(values)
+        if weight is not None:
+            t[5].copy_(weight)
+        e.teacher = (t, *how)
+
     def _record(self, e, x, y, lr, st):
         if lib.recorder is not None:        # another Trainer of this process is recording right now: this step runs as it is
             self._set_step_state(e, lr, 0)
@@ -275,6 +323,7 @@ class Trainer:
             e._plan_y = torch.empty_like(y, memory_format=torch.contiguous_format)
         e._plan_x.copy_(x)
         e._plan_y.copy_(y)
+        self._plan_teacher(e)
         self._set_step_state(e, lr, 0)
         plan = StepPlan()
         sig = self._host_signature(e)

@@ -22,7 +22,7 @@ from semseg_amd import distill as D
 ])
 def test_rows_of_a_tensor(make, dim, geom, strides, by_rows):
     z = make()
-    g = D._Geom(z, D._dim(z, dim))
+    g = D.Geom(z, D._dim(z, dim))
     assert (g.geom, g.strides, g.by_rows) == (geom, strides, by_rows)
     # every element is reached exactly where the strides say
     src = torch.arange(z.untyped_storage().nbytes() // 4)
@@ -153,3 +153,12 @@ def test_distill_gradient_formula_against_differences(tail, reduction):
     got = ref.distill(z, ids, top, T, tail, w, reduction, 0.0)[1][0]
     want = _differences(f, z)
     assert float((got - want).abs().max()) < 1e-6
+
+
+def test_a_teacher_answers_in_eval_mode_on_the_gpu_only():
+    from model.pspnet import PSPNet
+    m = PSPNet(layers=50, classes=5, pretrained=False)
+    with pytest.raises(RuntimeError, match="eval"):
+        m.train().top_logits(torch.zeros(1, 3, 9, 9), 2)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        m.eval().top_logits(torch.zeros(1, 3, 9, 9), 2)

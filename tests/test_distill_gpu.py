@@ -492,3 +492,107 @@ def test_a_teacher_and_its_student():
         close(last(z.grad, 1), gv, gb, "grad")
         with torch.no_grad():
             z -= 50 * z.grad
+
+
+# ---------------------------------------------------------------------------------------------
+# the training path
+# ---------------------------------------------------------------------------------------------
+def _net(seed, classes=21, dropout=0.0):
+    from model.pspnet import PSPNet
+    from oracle import segnet
+    torch.manual_seed(5)
+    m = PSPNet(layers=50, classes=classes, zoom_factor=8, dropout=dropout, pretrained=False)
+    m.load_state_dict(segnet.recipe_state_dict({k: tuple(v.shape) for k, v in m.state_dict().items()}, seed=seed))
+    return m.cuda()
+
+
+def test_top_logits_are_the_score_map_s():
+    m = _net(1234).eval()
+    x = torch.randn(2, 3, 73, 73, generator=torch.Generator().manual_seed(1)).cuda()
+    o = m.top_logits(x, 4, temperature=2.0)
+    assert o.top_ids.shape == o.top_logprobs.shape == (2, 4, 10, 10) and o.logprob is None
+    logits = m(x)                                        # align_corners=True: every 8th pixel (but for the grid's last) is a point of the map
+    eng = m._engine(x, False)
+    s = eng.scores_eval(x)
+    z = s.data[..., :21].movedim(-1, 1)
+    assert torch.allclose(logits[:, :, 0, 0], z[:, :, 0, 0], rtol=1e-5, atol=1e-5)
+    want = ref.logprobs(last(z, 1), None, 2.0, 4, 255)
+    assert torch.equal(last(o.top_ids, 1), want["top_ids"][0])
+    close(last(o.top_logprobs, 1), *want["top_logprobs"], "top_logprobs")
+    close(o.entropy, *want["entropy"], "entropy")
+    kept = o.top_ids.clone()
+    m.top_logits(x + 1, 4)
+    assert torch.equal(o.top_ids, kept)                  # new tensors, not the engine's buffers
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_trainer_distils_the_score_map(tail):
+    """The loss is the definition's on the step's own scores, and the scores' gradient is the cross entropy's plus distill_weight times the
+    definition's."""
+    from semseg_amd.trainer import Trainer
+    T, alpha = 2.0, 0.3
+    t, m = _net(77).eval(), _net(1234).train()
+    tr = Trainer(m, sync_bn=False, distill_weight=alpha, distill_temperature=T, distill_tail=tail)
+    tr.use_plan = False
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(2, 3, 73, 73, generator=gen).cuda()
+    y = torch.randint(0, 21, (2, 73, 73), generator=gen).cuda()
+    o = t.top_logits(x, 5, temperature=T if tail else 1.0)
+    w = (torch.rand(2, 10, 10, generator=gen) > 0.2).float().cuda()
+    assert len(tr.step(x, y, 0.0)) == 3                  # learning rate 0: the weights stay
+    e = tr.engine(x)
+    plain = e.grad_of(e._rec_main["scores"])[..., :21].double().cpu().clone()
+    before = e._rec_main["scores"].data[..., :21].double().cpu().clone()
+    pred, main, aux, kd = tr.step(x, y, 0.0, top=(o.top_ids, o.top_logprobs, w))
+    s = e._rec_main["scores"]
+    z = s.data[..., :21].double().cpu()
+    (lv, lb), (gv, gb) = ref.distill(z, last(o.top_ids, 1), last(o.top_logprobs, 1), T, tail, w.double().cpu(), "mean", HALF[torch.float32],
+                                     torch.tensor(alpha, dtype=torch.float64))
+    close(kd[0], lv, lb, "loss")
+    both = e.grad_of(s)[..., :21].double().cpu()
+    # the two steps' scores agree up to the merging order of the normalisations' statistics; so do the cross entropy's gradients
+    drift = float((z - before).abs().max())
+    assert drift < 1e-4
+    tol = gb + both.abs() * 2.0 ** -23 + plain.abs() * 2.0 ** -23 + 4 * drift * float(plain.abs().max()) + 1e-12
+    off = (both - plain - gv).abs()
+    assert bool((off <= tol).all()), float((off - tol).max())
+    assert float(e.grad_of(s)[..., 21:].abs().max()) == 0
+    for bad in ((o.top_ids[:1], o.top_logprobs[:1]), (o.top_ids, o.top_logprobs[:, :2]), (o.top_ids.float(), o.top_logprobs),
+                (o.top_ids, o.top_logprobs, w[:1])):
+        with pytest.raises((ValueError, TypeError)):
+            tr.step(x, y, 0.0, top=bad)
+    assert len(tr.step(x, y, 0.0)) == 3
+
+
+def test_replayed_distillation_steps_equal_eager_ones(report):
+    """Eight steps with a new batch, teacher's answer and learning rate each: replayed from the recorded step as launch by launch, inside 4x
+    the noise between two eager runs; a step without a teacher in between is not replayed from the record with one."""
+    from semseg_amd.trainer import Trainer
+
+    def run(plan):
+        t, m = _net(77).eval(), _net(1234, dropout=0.1).train()
+        tr = Trainer(m, sync_bn=False, distill_weight=0.5, distill_temperature=2.0)
+        tr.use_plan = plan
+        gen = torch.Generator().manual_seed(3)
+        losses = []
+        for it in range(8):
+            x = torch.randn(2, 3, 73, 73, generator=gen).cuda()
+            y = torch.randint(0, 21, (2, 73, 73), generator=gen).cuda()
+            o = t.top_logits(x, 4)
+            _, ml, al, kd = tr.step(x, y, 0.01 / (it + 1), top=(o.top_ids, o.top_logprobs))
+            losses.append((float(ml), float(al), float(kd)))
+        e = tr.engine(x)
+        return torch.tensor(losses), tr.flat_w.detach().cpu().clone(), tr, e, (x, y, o)
+    la, wa, _, _, _ = run(False)
+    lb, wb, _, _, _ = run(False)
+    lp, wp, tr, e, (x, y, o) = run(True)
+    assert e._plan is not None and e._plan_replays == 4, tr.plan_log
+    noise_l, noise_w = float((la - lb).abs().max()), float((wa - wb).abs().max())
+    off_l, off_w = float((lp - la).abs().max()), float((wp - wa).abs().max())
+    report("distillation steps replayed: losses off %.1e (eager twice %.1e), weights %.1e (%.1e)" % (off_l, noise_l, off_w, noise_w))
+    assert off_l <= 4 * noise_l + 1e-6 * float(la.abs().max()) and off_w <= 4 * noise_w + 1e-6 * float(wa.abs().max())
+    assert len(tr.step(x, y, 0.01)) == 3 and e._plan is None            # recorded again without the teacher
+    for _ in range(3):
+        out = tr.step(x, y, 0.01)
+    assert e._plan is not None and len(out) == 3
+    assert len(tr.step(x, y, 0.01, top=(o.top_ids, o.top_logprobs))) == 4 and e._plan is None
