@@ -254,7 +254,7 @@ struct Px {
 
 // ---- host side
 inline bool logits_ok(const void* z, int type, long long n, long long p, int C, float T) {
-  return z && type >= 0 && type <= 2 && n > 0 && p > 0 && C > 0 && C <= (1 << 30) && p <= (1ll << 40) / n && T > 0.f && T <= 3e38f;
+  return z && type >= 0 && type <= 2 && n > 0 && p > 0 && C > 0 && C <= (1 << 30) && p <= (1ll << 40) / n && T >= 1e-15f && T <= 1e15f;      // T^2 and 1 / T far from the ends of fp32
 }
 // rows: contiguous classes; planes: contiguous pixels (of fewer than 2^31 to an image)
 inline bool layout_ok(int C, long long p, long long sp, long long sc) { return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 31)); }

@@ -78,7 +78,8 @@ class Geom:
     def empty(self, size, dtype, device):
         """A dense tensor with `size` in the place of the classes, its rows laid out like the logits'."""
         if self.by_rows:
-            return torch.empty(self.shape + (size,), dtype=dtype, device=device).movedim(-1, self.dim)
+            t = torch.empty(self.shape + (size,), dtype=dtype, device=device)
+            return t if self.dim == len(self.shape) else t.movedim(-1, self.dim)
         return torch.empty(self.shape[:self.dim] + (size,) + self.shape[self.dim:], dtype=dtype, device=device)
 
     def dense(self, size):
@@ -96,14 +97,18 @@ class Geom:
         return (a[0][1] if a else 0, b[0][1] if b and self.p > 1 else 1, s)
 
 
+def check_temperature(temperature):
+    if not 1e-15 <= temperature <= 1e15:
+        raise ValueError("temperature must lie in [1e-15, 1e15], got %r" % (temperature,))
+
+
 def _check_logits(z, class_dim, temperature):
     if not isinstance(z, torch.Tensor) or z.dtype not in ops.TYPES:
         raise TypeError("logits must be an fp32, bf16 or fp16 tensor, got %s" % (z.dtype if isinstance(z, torch.Tensor) else type(z)))
     dim = _dim(z, class_dim)
     if z.numel() == 0:
         raise ValueError("logits of shape %s hold no value" % (tuple(z.shape),))
-    if not 0 < temperature < 3e38:
-        raise ValueError("temperature must be positive and finite, got %r" % (temperature,))
+    check_temperature(temperature)
     return Geom(z, dim)
 
 
@@ -198,7 +203,7 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255
 # ---------------------------------------------------------------------------------------------
 # distillation
 # ---------------------------------------------------------------------------------------------
-def _check_top(g, device, top_ids, top_values, weight):
+def check_top(g, device, top_ids, top_values, weight):
     """The teacher's entries of rows `g` on `device`, as the kernels take them."""
     if not isinstance(top_ids, torch.Tensor) or top_ids.dtype not in (torch.int32, torch.int64):
         raise TypeError("top_ids must be an int32 or int64 tensor")
@@ -232,7 +237,7 @@ def _check_top(g, device, top_ids, top_values, weight):
 
 def _check_distill(logits, top_ids, top_values, temperature, weight, class_dim, reduction, reductions):
     g = _check_logits(logits, class_dim, temperature)
-    teacher = _check_top(g, logits.device, top_ids, top_values, weight)
+    teacher = check_top(g, logits.device, top_ids, top_values, weight)
     if reduction not in reductions:
         raise ValueError("reduction must be one of %s, got %r" % (", ".join(reductions), reduction))
     _on_gpu(logits)

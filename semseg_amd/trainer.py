@@ -17,7 +17,7 @@ import torch.distributed as dist
 from . import engine as _engine
 from . import ops
 from ._lib import lib
-from .distill import Geom, _check_top
+from .distill import Geom, check_temperature, check_top
 from .engine import Engine
 from ._lib import debug
 from .plan import PlanError, StepPlan
@@ -140,10 +140,9 @@ class Trainer:
             h, w = e.score_hw()
             C = self.model.cls[4].weight.shape[0]
             rows = Geom(torch.empty(e.N, h, w, C, device="meta").movedim(-1, 1), 1)
-            e.teacher = (_check_top(rows, e.device, ids, values, weight), float(self.distill_temperature), bool(self.distill_tail),
+            check_temperature(self.distill_temperature)
+            e.teacher = (check_top(rows, e.device, ids, values, weight), float(self.distill_temperature), bool(self.distill_tail),
                          float(self.distill_weight))
-            if not 0 < e.teacher[1] < 3e38:
-                raise ValueError("distill_temperature must be positive and finite, got %r" % (self.distill_temperature,))
             sig = (tuple(ids.shape), ids.dtype, values.dtype, weight is None) + e.teacher[1:]
             e.distill_buffers()
         if sig != e._teacher_sig:         # what a recorded step bakes in of it (_host_signature)

@@ -57,6 +57,8 @@ def test_refusals():
         (lambda: D.class_logprobs(torch.zeros(2, 100), None, topk=65), ValueError),
         (lambda: D.class_logprobs(z, y, temperature=0.0), ValueError),
         (lambda: D.class_logprobs(z, y, temperature=math.inf), ValueError),
+        (lambda: D.class_logprobs(z, y, temperature=1e-16), ValueError),
+        (lambda: D.distill_loss(z, ids, top.detach(), temperature=1e16), ValueError),
         (lambda: D.class_logprobs(z, y, temperature=math.nan), ValueError),
         (lambda: D.class_logprobs(z[..., ::2], None), ValueError),
         (lambda: D.class_logprobs(torch.zeros(4, 10)[:, ::2], None), ValueError),
@@ -87,7 +89,7 @@ def test_the_c_entries_refuse_bad_arguments_without_a_gpu():
     fwd = lambda z=p, t=0, n=1, pp=4, C=8, T=1.0, k=0, lp=None, ids=None, lab=None: lib.semseg_class_logprobs_fwd(  # noqa: E731
         z, t, n, pp, C, *s3, lab, 255, T, k, lp, None, None, None, ids, ids, *none3, None, 0, None)
     for kw in (dict(z=None), dict(t=3), dict(t=-1), dict(n=0), dict(pp=0), dict(C=0), dict(T=0.0), dict(T=-1.0), dict(T=math.nan),
-               dict(T=math.inf), dict(k=-1), dict(k=1), dict(k=9, ids=p), dict(C=100, k=65, ids=p), dict(lp=p), dict(n=1 << 30, pp=1 << 30)):
+               dict(T=math.inf), dict(T=1e-16), dict(T=1e16), dict(k=-1), dict(k=1), dict(k=9, ids=p), dict(C=100, k=65, ids=p), dict(lp=p), dict(n=1 << 30, pp=1 << 30)):
         assert fwd(**kw) == -1, kw
     assert fwd(C=100000) == -1                  # one row in several slices needs scratch
     assert lib.semseg_class_logprobs_scratch_bytes(0, 1, 4, 8, 1, 5) == 0 < lib.semseg_class_logprobs_scratch_bytes(0, 1, 1, 100000, 1, 5)

@@ -24,7 +24,7 @@ ROWS = [
 PLANES = [
     ("planes", (1, 1, 1), 2, 0), ("planes", (2, 3, 5), 1, 0), ("planes", (2, 9, 7), 2, 0), ("planes", (1, 13, 11), 19, 0), ("planes", (3, 8, 8), 21, 0),
     ("planes", (2, 65, 65), 19, 0), ("planes", (1, 33, 31), 150, 0), ("planes", (2, 17, 15), 150, 0), ("planes", (2, 3, 5), 257, 0), ("planes", (1, 1, 3), 1000, 0),
-    ("planes", (1, 5, 1), 5000, 0), ("planes", (2, 8, 16), 40, 0),
+    ("planes", (1, 5, 1), 5000, 0), ("planes", (2, 8, 16), 40, 0), ("planes", (1, 2, 3), 9000, 0), ("planes", (1, 1, 2), 70001, 0),
 ]
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
@@ -442,6 +442,55 @@ def test_captured_graphs_replay_with_new_inputs():
             for _, out in graphs:
                 for k, (a, b) in enumerate(zip(out, want)):
                     assert torch.equal(a, b), (c, i, k)
+
+
+@pytest.mark.parametrize("C", [21, 150, 300, 4000])
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+def test_rows_that_two_strides_walk(C, dt):
+    """Cropped maps: rows of images that do not follow each other; alternatives, entries and gradients into such maps."""
+    gen = torch.Generator().manual_seed(20)
+    whole = torch.randn(3, 6, 5, C + 3, generator=gen).to(dt).to(DEV)
+    z = whole[:, 1:5, :, :C]
+    assert D.Geom(z, 3).geom == (3, 20, C)
+    y = labels((3, 4, 5), C, gen, ignore=-1)
+    o = check_logprobs(z, -1, y, 1.0, 6, ignore=-1)
+    zz = z.detach().requires_grad_()
+    o = D.class_logprobs(zz, y, ignore_index=-1, class_dim=-1)
+    g1 = torch.randn(3, 4, 5, generator=gen)
+    grad, = torch.autograd.grad(o.logprob, zz, g1.to(DEV))
+    v, b = ref.logprobs_grad(last(z, -1), y.cpu(), 1.0, -1, g1.double(), None, None, HALF[dt])
+    close(last(grad, -1), v, b, "grad", TINY[dt])
+    ids, top = teacher(("rows", (3, 4, 5), C, 3), z, -1, 5, 1.0, False, gen)
+    wide = torch.zeros(3, 9, 5, 5, dtype=torch.int32, device=DEV)
+    wide[:, 2:6] = ids
+    wtop = torch.zeros(3, 9, 5, 5, device=DEV)
+    wtop[:, 2:6] = top
+    for how in ("autograd", "fused"):
+        check_distill(z, -1, wide[:, 2:6], wtop[:, 2:6], 2.0, False, None, "mean", how)
+    out = torch.zeros_like(whole)
+    loss, _ = D.distill_loss_grad(z, ids, top, class_dim=-1, out=out[:, 1:5, :, :C])
+    loss2, g2 = D.distill_loss_grad(z, ids, top, class_dim=-1)
+    assert torch.equal(out[:, 1:5, :, :C], g2) and torch.equal(loss, loss2)
+    assert float(out[:, 0].abs().max()) == float(out[:, 5].abs().max()) == float(out[..., C:].abs().max()) == 0
+
+
+@pytest.mark.parametrize("case", [("rows", (6,), 21, 0), ("rows", (6,), 150, 0), ("rows", (6,), 1500, 0), ("rows", (6,), 9000, 0),
+                                  ("planes", (1, 2, 3), 21, 0), ("planes", (1, 2, 3), 150, 0)])
+@pytest.mark.parametrize("how", ["autograd", "fused"])
+def test_a_rest_far_below_the_entries(case, how):
+    """A student sure of the teacher's classes: what is outside them has a mass that fp32 does not hold, but a finite logarithm."""
+    gen = torch.Generator().manual_seed(21)
+    z, dim = make(case, torch.float32, gen)
+    zl = z.movedim(dim, -1).reshape(6, -1).clone()
+    ids = torch.stack([torch.randperm(case[2], generator=gen)[:3] for _ in range(6)]).to(DEV)
+    up = torch.tensor([[60.0], [120.0], [200.0], [400.0], [0.0], [1000.0]], device=DEV)
+    zl.scatter_add_(1, ids, up.expand(6, 3).contiguous())
+    top = torch.tensor([0.5, 0.2, 0.1], device=DEV).log().expand(6, 3).contiguous()
+    shape = z.movedim(dim, -1).shape
+    back = lambda t: t.view(shape[:-1] + (t.shape[-1],)).movedim(-1, dim).contiguous()  # noqa: E731
+    check_distill(back(zl), dim, back(ids), back(top), 1.0, True, None, "mean", how)
+    rows = D.distill_loss(back(zl), back(ids), back(top), tail=True, class_dim=dim, reduction="none").reshape(-1)
+    assert bool(torch.isfinite(rows).all()) and float(rows[5]) > 150
 
 
 def test_second_differentiation_is_refused():
