@@ -313,44 +313,51 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(const Logits a, const
   block_part<256>(o.part, loss, wsum);
 }
 
-// Longer rows: every block streams a slice and leaves its maximum and sum (with a tail: of the classes outside the entries, found by a
-// bitmap of the 16-byte chunks that hold one) ...
-constexpr int MAP_WORDS = 2048;
+// Longer rows: every block streams a slice and leaves its maximum and sum (with a tail: of the classes outside the entries.  A byte for
+// every 16-byte chunk says which of its classes the teacher names, a bit for every load of a wave whether one of its chunks has any, so
+// that most loads are done with a scalar test: 2048 x 131072 bf16, k 32: 160 us with a look at LDS for every chunk) ...
+constexpr int MAP_CHUNKS = 16384;
 struct DStream {
   long long r0;
   int nsplit, slice;
   float* part;               // [R][nsplit][2]
 };
-template <typename E>
+template <typename E, bool TAIL>
 __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, const Teacher t, const DStream d) {
   constexpr int V = VEC<E>, UN = 4;
-  __shared__ unsigned map[MAP_WORDS];
-  __shared__ int ids[MAXK];
+  __shared__ unsigned map[TAIL ? MAP_CHUNKS / 4 : 1];
+  __shared__ unsigned loads[4][2];           // of a wave: bit it of [it / 32]
   __shared__ float red[2][4];
   const int tid = threadIdx.x;
   const int sp = (int)(blockIdx.x % (unsigned)d.nsplit);
   const long long r = d.r0 + blockIdx.x / (unsigned)d.nsplit;
   if (t.weight && t.weight[r] == 0.f) return;
   const E* z = (const E*)a.z + a.at(r);
-  if (t.tail) {
-    const long long io = row_at(a, r, t.in, t.ip);
-    for (int j = tid; j < t.k; j += 256) {
-      const long long c = t.id(io, j);
-      ids[j] = c >= 0 && c < a.C ? (int)c : -1;
-    }
+  int id = -1;
+  if (TAIL && tid < t.k) {
+    const long long c = t.id(row_at(a, r, t.in, t.ip), tid);
+    id = c >= 0 && c < a.C ? (int)c : -1;
   }
   const int first = sp * d.slice, last = min(a.C, first + d.slice);
   float m = -INFINITY, s = 0.f, unused = 0.f;
-  for (int c0 = first; c0 < last; c0 += MAP_WORDS * 32 * V) {      // one turn up to 262144 classes
-    const int c1 = min(last, c0 + MAP_WORDS * 32 * V);
+  constexpr int TURN = TAIL ? MAP_CHUNKS * V : 1 << 30;
+  for (int c0 = first; c0 < last; c0 += TURN) {
+    const int c1 = last - c0 > TURN ? c0 + TURN : last;
     const int iters = (c1 - c0 + 256 * V - 1) / (256 * V);
-    if (t.tail) {
+    unsigned long long named = 0;
+    if (TAIL) {
       __syncthreads();
-      for (int i = tid; i < min(MAP_WORDS, iters * 8); i += 256) map[i] = 0;
+      for (int i = tid; i < iters * 64; i += 256) map[i] = 0;
+      if (tid < 8) loads[tid >> 1][tid & 1] = 0;
       __syncthreads();
-      for (int j = tid; j < t.k; j += 256)
-        if (ids[j] >= c0 && ids[j] < c1) atomicOr(&map[(ids[j] - c0) / V >> 5], 1u << ((ids[j] - c0) / V & 31));
+      if (id >= c0 && id < c1) {
+        const int ch = (id - c0) / V, c = c0 + ch * V, e = id - min(c, a.C - V);      // e: where load_chunk has it
+        atomicOr(&map[ch >> 2], 1u << ((ch & 3) * 8 + e));
+        atomicOr(&loads[(ch >> 6) & 3][ch >> 13], 1u << ((ch >> 8) & 31));
+      }
       __syncthreads();
+      named = (unsigned long long)__builtin_amdgcn_readfirstlane(loads[tid >> 6][1]) << 32 |
+              (unsigned)__builtin_amdgcn_readfirstlane(loads[tid >> 6][0]);
     }
     for (int it = 0; it < iters; it += UN) {
       float x[UN][V];
@@ -369,17 +376,15 @@ __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, con
           }
         }
       }
-      if (t.tail) {
+      if (TAIL && (named >> it & 15u)) {
 #pragma unroll
-        for (int n = 0; n < UN; ++n) {
-          const int ch = (it + n) * 256 + tid, c = c0 + ch * V;
-          if (c < c1 && (map[ch >> 5] >> (ch & 31) & 1u)) {
-            const int b = min(c, a.C - V);
-            for (int j = 0; j < t.k; ++j)
+        for (int n = 0; n < UN; ++n)
+          if (named >> (it + n) & 1u) {
+            const int ch = (it + n) * 256 + tid;
+            const unsigned in = map[ch >> 2] >> ((ch & 3) * 8);
 #pragma unroll
-              for (int e = 0; e < V; ++e) x[n][e] = ids[j] == b + e ? -INFINITY : x[n][e];
+            for (int e = 0; e < V; ++e) x[n][e] = in >> e & 1u ? -INFINITY : x[n][e];
           }
-        }
       }
       float nm = m;
 #pragma unroll
@@ -908,8 +913,11 @@ void distill_fwd(const Logits& a, const Teacher& t, const DistillOut& o, int typ
   const Split s = split_rows(type, a.R, a.C);
   DStream d{0, s.nsplit, s.slice, scratch};
   const long long most = (1ll << 23) / s.nsplit;
-  for (d.r0 = 0; d.r0 < a.R; d.r0 += most)
-    distill_stream_kernel<E><<<(int)(a.R - d.r0 < most ? a.R - d.r0 : most) * s.nsplit, 256, 0, stream>>>(a, t, d);
+  for (d.r0 = 0; d.r0 < a.R; d.r0 += most) {
+    const int blocks = (int)(a.R - d.r0 < most ? a.R - d.r0 : most) * s.nsplit;
+    if (t.tail) distill_stream_kernel<E, true><<<blocks, 256, 0, stream>>>(a, t, d);
+    else distill_stream_kernel<E, false><<<blocks, 256, 0, stream>>>(a, t, d);
+  }
   distill_join_kernel<E><<<blocks, 256, 0, stream>>>(a, t, o, d);
 }
 

@@ -493,6 +493,27 @@ def test_a_rest_far_below_the_entries(case, how):
     assert bool(torch.isfinite(rows).all()) and float(rows[5]) > 150
 
 
+@pytest.mark.parametrize("dt,C", [(torch.float32, 70001), (torch.bfloat16, 140003), (torch.float32, 150001)])
+def test_many_long_rows_as_few(dt, C):
+    """520 rows take a block each, 8 are sliced over many: the same rows either way (the latter are checked against the definition above);
+    long enough that a block turns to its map of the entries more than once, and that lines share a maximum."""
+    gen = torch.Generator().manual_seed(22)
+    z = (torch.randn(8, C, generator=gen) * 2).to(dt).to(DEV)
+    ids = torch.stack([torch.randperm(C, generator=gen)[:30] for _ in range(8)])
+    ids[:, 0], ids[:, 1] = C - 1, 0
+    top = torch.randn(8, 30, generator=gen).log_softmax(-1) - 0.3
+    ids, top, y = ids.to(DEV), top.to(DEV), torch.randint(0, C, (8,), generator=gen).to(DEV)
+    many = lambda t: t.repeat(65, *[1] * (t.dim() - 1))  # noqa: E731
+    few, all_ = (D.class_logprobs(a, b, topk=12, temperature=0.9, ignore_index=-1) for a, b in ((z, y), (many(z), many(y))))
+    assert torch.equal(many(few.top_ids), all_.top_ids)
+    for a, b in zip(few, all_):
+        assert torch.allclose(many(a), b, rtol=1e-5, atol=1e-5)
+    for tail in (True, False):
+        a = D.distill_loss(z, ids, top, tail=tail, reduction="none")
+        b = D.distill_loss(many(z), many(ids), many(top), tail=tail, reduction="none")
+        assert torch.allclose(many(a), b, rtol=1e-5, atol=1e-5) and bool((a > 0).all())
+
+
 def test_second_differentiation_is_refused():
     z = torch.randn(4, 9, device=DEV).requires_grad_()
     o = D.class_logprobs(z, torch.zeros(4, dtype=torch.int64, device=DEV))
