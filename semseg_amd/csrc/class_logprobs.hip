@@ -509,8 +509,9 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   __shared__ unsigned lists[SPLIT > 1 ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
   __shared__ int ids[SPLIT > 1 && IDS ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 && IDS ? 64 : 1];
   const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, pl = threadIdx.x & (LANES - 1);
-  const long long i = i0 + blockIdx.x / (unsigned)tiles;
-  const long long first = (long long)(blockIdx.x % (unsigned)tiles) * (LANES * PV) + pl * PV;
+  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
+  const long long i = i0 + bid / (unsigned)tiles;
+  const long long first = (long long)(bid % (unsigned)tiles) * (LANES * PV) + pl * PV;
   const Px<PV> px(first, a.p);
   const E* z = (const E*)a.z + i * a.sn + px.px;
   const int per = (a.C + SPLIT - 1) / SPLIT, c0 = wv * per, c1 = min(a.C, c0 + per);
@@ -762,8 +763,9 @@ template <typename E, int PV>
 __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a, const LogprobGrad g, const long long i0, const int tiles,
                                                                   const int slice) {
   constexpr int UN = 4;
-  const long long i = i0 + blockIdx.x / (unsigned)tiles;
-  const long long first = (long long)(blockIdx.x % (unsigned)tiles) * (256 * PV) + threadIdx.x * PV;
+  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
+  const long long i = i0 + bid / (unsigned)tiles;
+  const long long first = (long long)(bid % (unsigned)tiles) * (256 * PV) + threadIdx.x * PV;
   if (first >= a.p) return;
   const Px<PV> px(first, a.p);
   const E* z = (const E*)a.z + i * a.sn + px.px;

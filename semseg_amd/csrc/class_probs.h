@@ -190,7 +190,9 @@ __device__ __forceinline__ void rescale(float& s, float& u, float from, float to
   s = s * f;
 }
 
-// ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane
+// ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane.
+// Neighbouring tiles go to the same XCD (xcd_remap), so that what runs there at a time walks through one piece of every plane (the
+// distillation gradient of 4 x 150 x 473 x 473: 229 us, with tiles dealt out in turn 265).
 template <typename E, int PV>
 __device__ __forceinline__ void load_px(const E* p, E (&q)[PV]) {
   if constexpr (PV * sizeof(E) == 4) {

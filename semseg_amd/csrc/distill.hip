@@ -640,7 +640,7 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
   const int per = SPLIT > 1 ? ((a.C + SPLIT - 1) / SPLIT + CH - 1) / CH * CH : a.C;
   const int c_lo = wv * per, c_hi = min(a.C, c_lo + per);
   double loss = 0.0, wsum = 0.0;
-  for (long long it = blockIdx.x; it < all; it += gridDim.x) {
+  for (long long it = xcd_remap(blockIdx.x, gridDim.x); it < all; it += gridDim.x) {
     long long i = (long long)((double)it * inv_tiles), at = it - i * tiles;      // as in row_at
     if (at < 0) { --i; at += tiles; }
     if (at >= tiles) { ++i; at -= tiles; }
@@ -773,7 +773,8 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const Logits a, 
   constexpr int COLS = 64 * PV, UN = 8;
   __shared__ float tile[CH][COLS];
   const int lane = threadIdx.x;
-  const long long i = i0 + blockIdx.x / (unsigned)tiles, first = (long long)(blockIdx.x % (unsigned)tiles) * COLS + lane * PV;
+  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
+  const long long i = i0 + bid / (unsigned)tiles, first = (long long)(bid % (unsigned)tiles) * COLS + lane * PV;
   if (first >= a.p) return;
   const Px<PV> px(first, a.p);
   const E* z = (const E*)a.z + i * a.sn + px.px;
@@ -843,7 +844,7 @@ bool teacher_ok(const void* ids, int ids64, const void* top, int top_type, int k
 }
 
 // Blocks of the loss kernels: one partial sum each
-constexpr int PARTS = 4096;
+constexpr int PARTS = 16384;
 template <typename E>
 int distill_blocks(const Logits& a, long long* all, int* split) {
   if (a.C > 1 && a.sc != 1) {
