@@ -296,7 +296,7 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
 
 /* ---- class probabilities of logits (no counterpart in the reference): what a model answers with beyond its argmax, and what another
  * model learns from it.  A row is one pixel (or token) with C logits of type SEMSEG_TYPE_*; row i * p + j (i < n, j < p), class c, is
- * element i * sn + j * sp + c * sc (C <= 2^30, p < 2^31 where the pixels are contiguous, temperatures T of [1e-15, 1e15]), where the classes (sc = 1) or the pixels (sp = 1) are contiguous; a gradient has the same of its
+ * element i * sn + j * sp + c * sc (C <= 2^30, n * ceil(p / 64) < 2^31 where the pixels are contiguous, temperatures T of [1e-15, 1e15]), where the classes (sc = 1) or the pixels (sp = 1) are contiguous; a gradient has the same of its
  * strides equal to 1.  Every [n * p] operand is contiguous in that row order; results and sums are fp32.
  *
  * semseg_class_logprobs_fwd: log softmax(z / T) at the row's label (logprob; needs label), its entropy, lse = log sum exp(z / T), and

@@ -508,12 +508,14 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][4][PV][SPLIT > 1 ? 64 : 1];
   __shared__ unsigned lists[SPLIT > 1 ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 ? 64 : 1];
   __shared__ int ids[SPLIT > 1 && IDS ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 && IDS ? 64 : 1];
-  const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, pl = threadIdx.x & (LANES - 1);
-  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
-  const long long i = i0 + bid / (unsigned)tiles;
-  const long long first = (long long)(bid % (unsigned)tiles) * (LANES * PV) + pl * PV;
-  const Px<PV> px(first, a.p);
-  const E* z = (const E*)a.z + i * a.sn + px.px;
+  const int wv = SPLIT > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, pl = threadIdx.x & (LANES - 1);
+  unsigned image, at;
+  tile_of(xcd_remap(blockIdx.x, gridDim.x), tiles, image, at);
+  const long long i = i0 + image;
+  const Px<PV> px((long long)at * (LANES * PV), pl, a.p);
+  const E* zt = (const E*)a.z + i * a.sn + px.base;
+  const unsigned bytes = px.template bytes<E>();
+  const E* z = zt + (px.px - px.base);
   const int per = (a.C + SPLIT - 1) / SPLIT, c0 = wv * per, c1 = min(a.C, c0 + per);
   float m[PV], s[PV], u[PV], zy[PV];
   int yc[PV];
@@ -531,7 +533,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   // for memory at the same time.
   const auto load = [&](E(&q)[UN][PV], int c) {
 #pragma unroll
-    for (int n = 0; n < UN; ++n) load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, q[n]);
+    for (int n = 0; n < UN; ++n) load_px<E, PV>(zt + min(c + n, c1 - 1) * a.sc, bytes, q[n]);
   };
   const auto work = [&](const E(&q)[UN][PV], int c) {
     float x[UN][PV];
@@ -624,7 +626,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
       }
     }
   }
-  if (first >= a.p) return;
+  if (px.p0 >= a.p) return;
   const long long r = i * a.p + px.px, ot = i * o.tn + px.px * o.tp;
   float base[PV], ls[PV], out[PV];
   bool empty[PV], is_class[PV];
@@ -763,13 +765,14 @@ template <typename E, int PV>
 __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a, const LogprobGrad g, const long long i0, const int tiles,
                                                                   const int slice) {
   constexpr int UN = 4;
-  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
-  const long long i = i0 + bid / (unsigned)tiles;
-  const long long first = (long long)(bid % (unsigned)tiles) * (256 * PV) + threadIdx.x * PV;
-  if (first >= a.p) return;
-  const Px<PV> px(first, a.p);
-  const E* z = (const E*)a.z + i * a.sn + px.px;
-  E* dz = (E*)g.dz + i * g.dn + px.px;
+  unsigned image, at;
+  tile_of(xcd_remap(blockIdx.x, gridDim.x), tiles, image, at);
+  const long long i = i0 + image;
+  const Px<PV> px((long long)at * (256 * PV), threadIdx.x, a.p);
+  if (px.p0 >= a.p) return;
+  const E* z = (const E*)a.z + i * a.sn + px.base;
+  E* dz = (E*)g.dz + i * g.dn + px.base;
+  const unsigned bytes = px.template bytes<E>();
   RowGrad f[PV];
 #pragma unroll
   for (int v = 0; v < PV; ++v) f[v].init(a, g, i * a.p + px.px + v);
@@ -778,8 +781,8 @@ __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a
     E q[UN][PV], old[UN][PV];
 #pragma unroll
     for (int n = 0; n < UN; ++n) {
-      load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, q[n]);
-      if (g.accumulate) load_px<E, PV>(dz + min(c + n, c1 - 1) * g.dc, old[n]);
+      load_px<E, PV>(z + min(c + n, c1 - 1) * a.sc, bytes, q[n]);
+      if (g.accumulate) load_px<E, PV>(dz + min(c + n, c1 - 1) * g.dc, bytes, old[n]);
     }
 #pragma unroll
     for (int n = 0; n < UN; ++n) {
@@ -787,11 +790,11 @@ __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a
 #pragma unroll
       for (int v = 0; v < PV; ++v) q[n][v] = (E)(f[v](a, (float)q[n][v], c + n) + (g.accumulate ? (float)old[n][v] : 0.f));
       if (px.own(0)) {
-        store_px<E, PV>(dz + (c + n) * g.dc, q[n]);
+        store_px<E, PV>(dz + (c + n) * g.dc, bytes, q[n]);
       } else {
 #pragma unroll
         for (int v = 1; v < PV; ++v)
-          if (px.own(v)) store1(dz + (c + n) * g.dc + v, (float)q[n][v]);
+          if (px.own(v)) store_at(dz + (c + n) * g.dc + v, bytes, q[n][v]);
       }
     }
   }
@@ -912,7 +915,7 @@ int semseg_class_logprobs_fwd(const void* z, int type, long long n, long long p,
                               void* scratch, size_t scratch_bytes, hipStream_t stream) {
   if (!logits_ok(z, type, n, p, C, T) || k < 0 || k > MAXK || k > C || (k && (!top_ids || !top_logprobs)) || (logprob && !label))
     return SEMSEG_EINVAL;
-  if (!layout_ok(C, p, sp, sc)) return SEMSEG_EINVAL;
+  if (!layout_ok(C, n, p, sp, sc)) return SEMSEG_EINVAL;
   const size_t need = semseg_class_logprobs_scratch_bytes(type, n, p, C, sc, k);
   if (need && (!scratch || scratch_bytes < need)) return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
@@ -927,7 +930,7 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
                               long long dp, long long dc, int accumulate, hipStream_t stream) {
   if (!logits_ok(z, type, n, p, C, T) || !stats || !dz || (g_entropy && !entropy) || (g_logprob && !label)) return SEMSEG_EINVAL;
   // the gradient is in the logits' form
-  if (!layout_ok(C, p, sp, sc) || !(C == 1 || (sc == 1 ? dc == 1 : dp == 1))) return SEMSEG_EINVAL;
+  if (!layout_ok(C, n, p, sp, sc) || !(C == 1 || (sc == 1 ? dc == 1 : dp == 1))) return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
   const LogprobGrad g{label, ignore_index, stats, entropy, g_logprob, g_entropy, g_lse, dz, dn, dp, dc, accumulate};
   BY_TYPE(type, logprobs_bwd, a, g, stream);

@@ -193,59 +193,50 @@ __device__ __forceinline__ void rescale(float& s, float& u, float from, float to
 // ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane.
 // Neighbouring tiles go to the same XCD (xcd_remap), so that what runs there at a time walks through one piece of every plane (the
 // distillation gradient of 4 x 150 x 473 x 473: 229 us, with tiles dealt out in turn 265).
+// A lane's address is a wave-uniform plane and 32 bits of its own: no 64-bit addresses in vector registers.
+template <typename T>
+__device__ __forceinline__ T load_at(const void* plane, unsigned bytes) {
+  struct __attribute__((packed, aligned(2))) W { T v; };
+  return reinterpret_cast<const W*>(static_cast<const char*>(plane) + bytes)->v;
+}
+template <typename T>
+__device__ __forceinline__ void store_at(void* plane, unsigned bytes, T v) {
+  struct __attribute__((packed, aligned(2))) W { T v; };
+  reinterpret_cast<W*>(static_cast<char*>(plane) + bytes)->v = v;
+}
+template <int BYTES> struct Word;
+template <> struct Word<2> { using type = unsigned short; };
+template <> struct Word<4> { using type = unsigned; };
+template <> struct Word<8> { using type = u32x2; };
 template <typename E, int PV>
-__device__ __forceinline__ void load_px(const E* p, E (&q)[PV]) {
-  if constexpr (PV * sizeof(E) == 4) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
-    const unsigned w = reinterpret_cast<const W*>(p)->v;
-    __builtin_memcpy(q, &w, 4);
-  } else if constexpr (PV * sizeof(E) == 8) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
-    const u32x2 w = reinterpret_cast<const W*>(p)->v;
-    __builtin_memcpy(q, &w, 8);
-  } else if constexpr (PV * sizeof(E) == 16) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { u32x4 v; };
-    const u32x4 w = reinterpret_cast<const W*>(p)->v;
-    __builtin_memcpy(q, &w, 16);
-  } else {
-#pragma unroll
-    for (int v = 0; v < PV; ++v) q[v] = p[v];
-  }
+__device__ __forceinline__ void load_px(const E* plane, unsigned bytes, E (&q)[PV]) {
+  const auto w = load_at<typename Word<PV * sizeof(E)>::type>(plane, bytes);
+  __builtin_memcpy(q, &w, sizeof(w));
 }
 template <typename E, int PV>
-__device__ __forceinline__ void store_px(E* p, const E (&q)[PV]) {
-  if constexpr (PV * sizeof(E) == 4) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { unsigned v; };
-    unsigned w;
-    __builtin_memcpy(&w, q, 4);
-    reinterpret_cast<W*>(p)->v = w;
-  } else if constexpr (PV * sizeof(E) == 8) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { u32x2 v; };
-    u32x2 w;
-    __builtin_memcpy(&w, q, 8);
-    reinterpret_cast<W*>(p)->v = w;
-  } else if constexpr (PV * sizeof(E) == 16) {
-    struct __attribute__((packed, aligned(alignof(E)))) W { u32x4 v; };
-    u32x4 w;
-    __builtin_memcpy(&w, q, 16);
-    reinterpret_cast<W*>(p)->v = w;
-  } else {
-#pragma unroll
-    for (int v = 0; v < PV; ++v) p[v] = q[v];
-  }
+__device__ __forceinline__ void store_px(E* plane, unsigned bytes, const E (&q)[PV]) {
+  typename Word<PV * sizeof(E)>::type w;
+  __builtin_memcpy(&w, q, sizeof(w));
+  store_at(plane, bytes, w);
 }
-// Pixels of a tile of lanes: lane `pl` of tile `t` has PV pixels from `px` on, those from `p0` on are its own (an image's last lane is
-// moved back so that it loads whole pieces).
+// Pixels of a tile that starts at pixel t0: lane `pl` has PV pixels from `px` on, those from `p0` on are its own (an image's last lane is
+// moved back so that it loads whole pieces); `base` is a pixel that no lane of the tile is before.
 template <int PV>
 struct Px {
-  long long px, p0, P;
-  __device__ __forceinline__ Px(long long first, long long P_) : px(first < P_ - PV ? first : P_ - PV), p0(first), P(P_) {}
+  long long px, p0, base;
+  __device__ __forceinline__ Px(long long t0, int pl, long long P) {
+    p0 = t0 + pl * PV;
+    px = p0 < P - PV ? p0 : P - PV;
+    base = t0 < PV ? 0 : t0 - PV;
+  }
   __device__ __forceinline__ bool own(int v) const { return px + v >= p0; }
+  template <typename T>
+  __device__ __forceinline__ unsigned bytes() const { return (unsigned)(px - base) * (unsigned)sizeof(T); }
   // the own values of `x` to p, p + step, ...: together where they lie side by side
   template <typename T>
   __device__ __forceinline__ void put(T* p, long long step, const T (&x)[PV]) const {
     if (step == 1 && own(0)) {
-      store_px<T, PV>(p, x);
+      store_px<T, PV>(p, 0, x);
     } else {
 #pragma unroll
       for (int v = 0; v < PV; ++v)
@@ -253,13 +244,20 @@ struct Px {
     }
   }
 };
+// tile and image of a block
+__device__ __forceinline__ void tile_of(unsigned bid, int tiles, unsigned& image, unsigned& tile) {
+  image = __builtin_amdgcn_readfirstlane(bid / (unsigned)tiles);
+  tile = __builtin_amdgcn_readfirstlane(bid - image * (unsigned)tiles);
+}
 
 // ---- host side
 inline bool logits_ok(const void* z, int type, long long n, long long p, int C, float T) {
   return z && type >= 0 && type <= 2 && n > 0 && p > 0 && C > 0 && C <= (1 << 30) && p <= (1ll << 40) / n && T >= 1e-15f && T <= 1e15f;      // T^2 and 1 / T far from the ends of fp32
 }
-// rows: contiguous classes; planes: contiguous pixels (of fewer than 2^31 to an image)
-inline bool layout_ok(int C, long long p, long long sp, long long sc) { return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 31)); }
+// rows: contiguous classes; planes: contiguous pixels, and fewer than 2^31 tiles of 64 pixels
+inline bool layout_ok(int C, long long n, long long p, long long sp, long long sc) {
+  return C == 1 || sc == 1 || (sp == 1 && p < (1ll << 31) && n < (1ll << 31) / ((p + 63) / 64));
+}
 inline Logits logits_of(const void* z, long long n, long long p, int C, long long sn, long long sp, long long sc, float T) {
   return Logits{z, n * p, p, sn, sp, sc, C, 1.f / T, LOG2E / T, 1.0 / (double)p};
 }

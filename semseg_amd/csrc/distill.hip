@@ -631,22 +631,23 @@ struct PixTeacher {
 // with SPLIT = 4 four waves share them and take a quarter of the classes each.
 template <typename E, int PV, int KR, int SPLIT, bool TAIL>
 __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits a, const Teacher t, const DistillOut o, const int tiles,
-                                                                    const long long all, const double inv_tiles) {
+                                                                    const long long all) {
   constexpr int COLS = 64 * PV;
   __shared__ float tiles_s[SPLIT][CH][COLS];
   __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][5][SPLIT > 1 ? COLS : 1];
-  const int wv = SPLIT > 1 ? threadIdx.x >> 6 : 0, lane = threadIdx.x & 63;
+  const int wv = SPLIT > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, lane = threadIdx.x & 63;
   float(*tile)[COLS] = tiles_s[wv];
   const int per = SPLIT > 1 ? ((a.C + SPLIT - 1) / SPLIT + CH - 1) / CH * CH : a.C;
   const int c_lo = wv * per, c_hi = min(a.C, c_lo + per);
   double loss = 0.0, wsum = 0.0;
   for (long long it = xcd_remap(blockIdx.x, gridDim.x); it < all; it += gridDim.x) {
-    long long i = (long long)((double)it * inv_tiles), at = it - i * tiles;      // as in row_at
-    if (at < 0) { --i; at += tiles; }
-    if (at >= tiles) { ++i; at -= tiles; }
-    const long long first = at * COLS + lane * PV;
-    const Px<PV> px(first, a.p);
-    const E* z = (const E*)a.z + i * a.sn + px.px;
+    unsigned image, at;
+    tile_of((unsigned)it, tiles, image, at);
+    const long long i = image;
+    const Px<PV> px((long long)at * COLS, lane, a.p);
+    const E* zt = (const E*)a.z + i * a.sn + px.base;
+    const unsigned bytes = px.template bytes<E>();
+    const E* z = zt + (px.px - px.base);
     const long long r0 = i * a.p + px.px, io = i * t.in + px.px * t.ip, vo = i * t.vn + px.px * t.vp;
     float m[PV], base[PV], s[PV], st[PV], dot[PV], qacc[PV];
     PixTeacher<KR> q[PV];
@@ -659,7 +660,7 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       E x[CH][PV];
 #pragma unroll
-      for (int n = 0; n < CH; ++n) load_px<E, PV>(z + min(c0 + n, c_hi - 1) * a.sc, x[n]);
+      for (int n = 0; n < CH; ++n) load_px<E, PV>(zt + min(c0 + n, c_hi - 1) * a.sc, bytes, x[n]);
 #pragma unroll
       for (int v = 0; v < PV; ++v) {
         float y[CH], nm = m[v];
@@ -720,7 +721,7 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
         }
       }
     }
-    if (first >= a.p) continue;
+    if (px.p0 >= a.p) continue;
     float s0[PV], s1[PV], s2[PV], lr[PV];
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
@@ -773,12 +774,14 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const Logits a, 
   constexpr int COLS = 64 * PV, UN = 8;
   __shared__ float tile[CH][COLS];
   const int lane = threadIdx.x;
-  const unsigned bid = xcd_remap(blockIdx.x, gridDim.x);
-  const long long i = i0 + bid / (unsigned)tiles, first = (long long)(bid % (unsigned)tiles) * COLS + lane * PV;
-  if (first >= a.p) return;
-  const Px<PV> px(first, a.p);
-  const E* z = (const E*)a.z + i * a.sn + px.px;
-  E* dz = (E*)g.dz + i * g.dn + px.px;
+  unsigned image, at;
+  tile_of(xcd_remap(blockIdx.x, gridDim.x), tiles, image, at);
+  const long long i = i0 + image;
+  const Px<PV> px((long long)at * COLS, lane, a.p);
+  if (px.p0 >= a.p) return;
+  const E* z = (const E*)a.z + i * a.sn + px.base;
+  E* dz = (E*)g.dz + i * g.dn + px.base;
+  const unsigned bytes = px.template bytes<E>();
   const long long r0 = i * a.p + px.px, io = i * t.in + px.px * t.ip, vo = i * t.vn + px.px * t.vp;
   PixTeacher<KR> q[PV];
   float base[PV], ls2[PV], off2[PV], cq[PV], f[PV], coef[PV];
@@ -813,8 +816,8 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const Logits a, 
       E x[UN][PV], old[UN][PV];
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
-        load_px<E, PV>(z + min(c0 + h + n, c_hi - 1) * a.sc, x[n]);
-        if (g.accumulate) load_px<E, PV>(dz + min(c0 + h + n, c_hi - 1) * g.dc, old[n]);
+        load_px<E, PV>(z + min(c0 + h + n, c_hi - 1) * a.sc, bytes, x[n]);
+        if (g.accumulate) load_px<E, PV>(dz + min(c0 + h + n, c_hi - 1) * g.dc, bytes, old[n]);
       }
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
@@ -828,11 +831,11 @@ __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const Logits a, 
           x[n][v] = (E)(y + (g.accumulate ? (float)old[n][v] : 0.f));
         }
         if (px.own(0)) {
-          store_px<E, PV>(dz + (c0 + h + n) * g.dc, x[n]);
+          store_px<E, PV>(dz + (c0 + h + n) * g.dc, bytes, x[n]);
         } else {
 #pragma unroll
           for (int v = 1; v < PV; ++v)
-            if (px.own(v)) store1(dz + (c0 + h + n) * g.dc + v, (float)x[n][v]);
+            if (px.own(v)) store_at(dz + (c0 + h + n) * g.dc + v, bytes, x[n][v]);
         }
       }
     }
@@ -894,8 +897,8 @@ void distill_fwd(const Logits& a, const Teacher& t, const DistillOut& o, int typ
     const int pv = a.p >= PV ? PV : 1, tiles = (int)((a.p + 64 * pv - 1) / (64 * pv));
 #define DPLANES(PV_, KR, SP)                                                                                              \
   do {                                                                                                                    \
-    if (t.tail) distill_planes_kernel<E, PV_, KR, SP, true><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all, 1.0 / tiles);         \
-    else distill_planes_kernel<E, PV_, KR, SP, false><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all, 1.0 / tiles);               \
+    if (t.tail) distill_planes_kernel<E, PV_, KR, SP, true><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all);         \
+    else distill_planes_kernel<E, PV_, KR, SP, false><<<blocks, 64 * SP, 0, stream>>>(a, t, o, tiles, all);               \
   } while (0)
     if (PV > 1 && pv == 1) DPLANES(1, 0, 4);
     else if (split == 1 && t.k <= 4) DPLANES(PV, 4, 1);
@@ -974,7 +977,7 @@ int semseg_distill_fwd(const void* z, int type, long long n, long long p, int C,
                        int ids64, const void* top, int top_type, int k, long long in, long long ip, long long ik, long long vn,
                        long long vp, long long vk, const float* weight, float T, int tail, int reduction, float* rows, float* stats,
                        double* acc2, float* loss, void* scratch, size_t scratch_bytes, hipStream_t stream) {
-  if (!logits_ok(z, type, n, p, C, T) || !layout_ok(C, p, sp, sc) || !teacher_ok(ids, ids64, top, top_type, k) || !stats || reduction < 0 ||
+  if (!logits_ok(z, type, n, p, C, T) || !layout_ok(C, n, p, sp, sc) || !teacher_ok(ids, ids64, top, top_type, k) || !stats || reduction < 0 ||
       reduction > 2 || !scratch || scratch_bytes < distill_need(type, n * p, C, sc) ||
       (reduction == SEMSEG_REDUCE_NONE ? !rows : (!acc2 || !loss)))
     return SEMSEG_EINVAL;
@@ -996,7 +999,7 @@ int semseg_distill_bwd(const void* z, int type, long long n, long long p, int C,
                        long long vp, long long vk, const float* weight, float T, int tail, int reduction, const float* stats,
                        const double* acc2, const float* grad_loss, float grad_mul, void* dz, long long dn, long long dp, long long dc,
                        int accumulate, hipStream_t stream) {
-  if (!logits_ok(z, type, n, p, C, T) || !layout_ok(C, p, sp, sc) || !teacher_ok(ids, ids64, top, top_type, k) || !stats || !dz ||
+  if (!logits_ok(z, type, n, p, C, T) || !layout_ok(C, n, p, sp, sc) || !teacher_ok(ids, ids64, top, top_type, k) || !stats || !dz ||
       reduction < 0 || reduction > 2 || (reduction == SEMSEG_REDUCE_MEAN && !acc2) || !(C == 1 || (sc == 1 ? dc == 1 : dp == 1)))
     return SEMSEG_EINVAL;
   const Logits a = logits_of(z, n, p, C, sn, sp, sc, T);
