@@ -191,8 +191,8 @@ __device__ __forceinline__ void rescale(float& s, float& u, float from, float to
 }
 
 // ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane.
-// Neighbouring tiles go to the same XCD (xcd_remap), so that what runs there at a time walks through one piece of every plane (the
-// distillation gradient of 4 x 150 x 473 x 473: 229 us, with tiles dealt out in turn 265).
+// Where planes are written, or a tile is a single wave, neighbouring tiles go to the same XCD (xcd_remap), so that what runs there at a
+// time walks through one piece of every plane (the distillation gradient of 4 x 150 x 473 x 473: 229 us, with tiles dealt out in turn 265).
 // A lane's address is a wave-uniform plane and 32 bits of its own: no 64-bit addresses in vector registers.
 template <typename T>
 __device__ __forceinline__ T load_at(const void* plane, unsigned bytes) {
