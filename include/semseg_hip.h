@@ -296,15 +296,16 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
 
 /* ---- class probabilities of logits (no counterpart in the reference): what a model answers with beyond its argmax, and what another
  * model learns from it.  A row is one pixel (or token) with C logits of type SEMSEG_TYPE_*; row i * p + j (i < n, j < p), class c, is
- * element i * sn + j * sp + c * sc (C <= 2^30, n * ceil(p / 64) < 2^31 where the pixels are contiguous, temperatures T of [1e-15, 1e15]), where the classes (sc = 1) or the pixels (sp = 1) are contiguous; a gradient has the same of its
- * strides equal to 1.  Every [n * p] operand is contiguous in that row order; results and sums are fp32.
+ * element i * sn + j * sp + c * sc, where the classes (sc = 1) or the pixels (sp = 1) are contiguous; a gradient has the same of its
+ * strides equal to 1.  C <= 2^30, n * ceil(p / 64) < 2^31 where the pixels are contiguous, temperatures T of [1e-15, 1e15].  Every
+ * [n * p] operand is contiguous in that row order; results and sums are fp32.
  *
  * semseg_class_logprobs_fwd: log softmax(z / T) at the row's label (logprob; needs label), its entropy, lse = log sum exp(z / T), and
  * the k <= SEMSEG_CLASS_TOP_MAX classes of the largest logits with their log probabilities, in falling order, equal logits by rising
  * class; row (i, j)'s alternative a is element i * tn + j * tp + a * tk of top_ids / top_logprobs.  Any output may be NULL.  stats
  * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
  * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
- * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes), nothing needs to be cleared.
+ * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes) aligned to 8, nothing needs to be cleared.
  * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (its alternatives: NaN and +inf first, by class).
  * semseg_class_logprobs_bwd: dz (=|+=) the gradient from those of logprob, entropy, lse (each may be NULL); 0 for rows that are void
  * or hold only -inf; strides dn, dp, dc; dz has the logits' type, one rounding. */
@@ -328,7 +329,7 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
  * with p = softmax(z / T).  rows: T^2 * weight_r * loss_r (needed by SEMSEG_REDUCE_NONE, else may be NULL).  loss: their sum (SUM),
  * over the sum of weights (MEAN; NaN where that is 0, like an all-void cross entropy; gradients 0).  weight NULL: 1; rows of weight 0
  * are not read.  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
- * semseg_distill_scratch_bytes() bytes, nothing needs to be cleared; no atomics, results do not depend on scheduling.
+ * semseg_distill_scratch_bytes() bytes aligned to 8, nothing needs to be cleared; no atomics, results do not depend on scheduling.
  * _bwd: dz (=|+=) grad_mul * grad_loss (one device float, one per row for NONE, NULL: 1) * d loss / dz.
  * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call; stats may be NULL for rows of contiguous classes up to
  * SEMSEG_ROW_CLASSES. */

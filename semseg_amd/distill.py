@@ -180,12 +180,12 @@ class _Logprobs(torch.autograd.Function):
         return dz, None, None, None, None, None
 
 
-def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255, class_dim=1):
+def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=None, class_dim=1):
     """Log softmax(logits / temperature) at the rows' labels, its entropy and log-sum-exp, and the `topk` best classes of every row
     with their log probabilities (falling, equal logits by rising class).  logprob, entropy and lse carry gradients.
 
-    label: int64, the logits' shape without the classes.  Rows labelled ignore_index are void: not read, zero outputs, no alternatives
-    (ids -1, log probabilities -inf), zero gradient.  A label that is neither gives log probability NaN (ops.label_check counts them).
+    label: int64, the logits' shape without the classes.  Rows labelled ignore_index (default: 255, as in the segmentation losses, where
+    that is no class, otherwise -100) are void: not read, zero outputs, no alternatives (ids -1, log probabilities -inf), zero gradient.  A label that is neither gives log probability NaN (ops.label_check counts them).
     A row of -inf logits has log probabilities -inf, entropy 0 and no gradient."""
     g = _check_logits(logits, class_dim, temperature)
     if label is not None:
@@ -193,6 +193,8 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=255
         label = label.contiguous()
     if isinstance(topk, bool) or not isinstance(topk, int) or not 0 <= topk <= min(TOP_MAX, g.C):
         raise ValueError("topk must be a whole number of [0, min(%d, classes = %d)], got %r" % (TOP_MAX, g.C, topk))
+    if ignore_index is None:
+        ignore_index = 255 if g.C <= 255 else -100
     _on_gpu(logits)
     if logits.requires_grad and torch.is_grad_enabled():
         return ClassLogprobs(*_Logprobs.apply(logits, g, label, int(ignore_index), float(temperature), topk))
@@ -245,38 +247,34 @@ def _check_distill(logits, top_ids, top_values, temperature, weight, class_dim, 
 
 
 def _distill(z, g, teacher, temperature, tail, reduction):
-    dev, rows, acc, loss = z.device, None, None, None
-    stats = torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
-    if reduction == "none":
-        rows = torch.empty(g.shape, dtype=torch.float32, device=dev)
-    else:
-        acc, loss = torch.empty(2, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-    scratch = torch.empty(ops.distill_scratch_bytes(z.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
-    ids, ids_s, top, top_s, k, weight = teacher
-    ops.distill_fwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, rows, stats, acc, loss, scratch)
-    return (rows if loss is None else loss), stats, acc
+    """(loss or losses of the rows, workspace, its offsets)"""
+    nbytes, at = ops.distill_workspace(z.dtype, *g.geom, g.strides[2])
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=z.device)
+    out = torch.empty(g.shape if reduction == "none" else (), dtype=torch.float32, device=z.device)
+    rows, loss = (out, None) if reduction == "none" else (None, out)
+    ops.distill_fwd(z, g.geom, g.strides, *teacher, temperature, tail, reduction, rows, loss, ws, at)
+    return out, ws, at
 
 
 class _Distill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, g, teacher, temperature, tail, reduction):
         with _on_device(z):
-            loss, stats, acc = _distill(z, g, teacher, temperature, tail, reduction)
+            loss, ws, at = _distill(z, g, teacher, temperature, tail, reduction)
         ids, ids_s, top, top_s, k, weight = teacher
-        ctx.save_for_backward(z, ids, top, weight, stats, acc)
-        ctx.g, ctx.how = g, (ids_s, top_s, k, temperature, tail, reduction)
+        ctx.save_for_backward(z, ids, top, weight, ws)
+        ctx.how = g, ids_s, top_s, k, temperature, tail, reduction, at
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        z, ids, top, weight, stats, acc = ctx.saved_tensors
-        g = ctx.g
-        ids_s, top_s, k, temperature, tail, reduction = ctx.how
+        z, ids, top, weight, ws = ctx.saved_tensors
+        g, ids_s, top_s, k, temperature, tail, reduction, at = ctx.how
         with _on_device(z):
             dz = g.empty(g.C, z.dtype, z.device)
-            ops.distill_bwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, stats, acc,
-                            grad.contiguous(), 1.0, dz, g.dense(g.C))
+            ops.distill_bwd(z, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, ws, at, grad.contiguous(),
+                            1.0, dz, g.dense(g.C))
         return dz, None, None, None, None, None
 
 
@@ -320,10 +318,8 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
             raise ValueError("out of strides %s does not have the logits' layout" % (tuple(out.stride()),))
     with _on_device(logits):
         # rows that fit registers need no statistics kept for a second pass
-        stats = None if g.by_rows and g.C <= ops.ROW_CLASSES else torch.empty((3,) + g.shape, dtype=torch.float32, device=dev)
-        acc, loss = torch.empty(2, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
-        scratch = torch.empty(ops.distill_scratch_bytes(logits.dtype, *g.geom, g.strides[2]), dtype=torch.uint8, device=dev)
-        ids, ids_s, top, top_s, k, weight = teacher
-        ops.distill_fwd_bwd(logits, g.geom, g.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, reduction, stats, acc, loss,
-                            grad_scale, out, ds, accumulate, scratch)
+        nbytes, at = ops.distill_workspace(logits.dtype, *g.geom, g.strides[2], stats=not (g.by_rows and g.C <= ops.ROW_CLASSES))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        ops.distill_fwd_bwd(logits, g.geom, g.strides, *teacher, temperature, tail, reduction, loss, grad_scale, out, ds, accumulate, ws, at)
     return loss, out

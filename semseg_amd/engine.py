@@ -1308,22 +1308,22 @@ class Engine:
         if self._distill_bufs is None:
             C = self.model.cls[4].weight.shape[0]
             h, w = self.score_hw()
-            new = lambda n, dt: torch.empty(n, dtype=dt, device=self.device)  # noqa: E731
-            self._distill_bufs = dict(loss=new(1, F32), acc=new(2, F64), stats=new(3 * self.N * h * w, F32),
-                                      scratch=new(ops.distill_scratch_bytes(F32, 1, self.N * h * w, C, 1), torch.uint8))
+            nbytes, at = ops.distill_workspace(F32, 1, self.N * h * w, C, 1)
+            self._distill_bufs = dict(loss=torch.empty(1, dtype=F32, device=self.device), at=at,
+                                      ws=torch.empty(nbytes, dtype=torch.uint8, device=self.device))
         return self._distill_bufs
 
     def distill_bwd(self):
         """Distillation from the teacher's top classes on the main scores, loss and gradient in one pass over them: d scores +=
         factor * d(T^2 KL(teacher || scores)) / d scores, behind the cross entropy's, which writes that buffer."""
-        (ids, ids_s, top, top_s, k, weight), temperature, tail, factor = self.teacher
+        entries, temperature, tail, factor = self.teacher
         s = self._rec_main["scores"]
         g = self.grad_of(s)
         assert s.ginit
         rows = Geom(s.data[..., :s.C].movedim(-1, 1), 1)
         b = self.distill_buffers()
-        ops.distill_fwd_bwd(s.data, rows.geom, rows.strides, ids, ids_s, top, top_s, k, weight, temperature, tail, "mean", b["stats"],
-                            b["acc"], b["loss"], factor, g, rows.strides, True, b["scratch"])
+        ops.distill_fwd_bwd(s.data, rows.geom, rows.strides, *entries, temperature, tail, "mean", b["loss"], factor, g, rows.strides, True,
+                            b["ws"], b["at"])
 
     # ------------------------------------------------------------------ whole-network passes
     def score_hw(self):

@@ -606,28 +606,43 @@ def _teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction):
             int(tail), REDUCTIONS[reduction])
 
 
-def distill_fwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, rows, stats, acc2, loss, scratch):
+def distill_workspace(dtype, n, p, C, sc, stats=True):
+    """(bytes, offsets) of one buffer for a call's accumulators, scratch and (stats) row statistics: the three operands that are nobody
+    else's.  The offsets are passed on as `at` below."""
+    scratch = distill_scratch_bytes(dtype, n, p, C, sc)
+    return 16 + scratch + (12 * n * p if stats else 0), (0, 16, 16 + scratch if stats else None)
+
+
+def _work(ws, at):
+    """acc2, scratch, stats of a workspace tensor."""
+    base = ws.data_ptr()
+    return base + at[0], base + at[1], None if at[2] is None else base + at[2]
+
+
+def distill_fwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, rows, loss, ws, at):
+    acc, scratch, stats = _work(ws, at)
     _ck(lib.semseg_distill_fwd(_p(z), TYPES[z.dtype], *geom, *strides,
-                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(rows), _p(stats),
-                               _p(acc2), _p(loss), _p(scratch), 0 if scratch is None else scratch.numel() * scratch.element_size(),
-                               _stream()), "distill_fwd")
+                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(rows), stats, acc, _p(loss),
+                               scratch, at[2] - at[1], _stream()), "distill_fwd")
 
 
-def distill_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, stats, acc2, grad_loss, grad_mul,
-                dz, dstrides, accumulate=False):
+def distill_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, ws, at, grad_loss, grad_mul, dz,
+                dstrides, accumulate=False):
     assert dz.dtype == z.dtype
+    acc, _, stats = _work(ws, at)
     _ck(lib.semseg_distill_bwd(_p(z), TYPES[z.dtype], *geom, *strides,
-                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(stats), _p(acc2),
-                               _p(grad_loss), float(grad_mul), _p(dz), *dstrides, int(accumulate), _stream()), "distill_bwd")
+                               *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), stats, acc, _p(grad_loss),
+                               float(grad_mul), _p(dz), *dstrides, int(accumulate), _stream()), "distill_bwd")
 
 
-def distill_fwd_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, stats, acc2, loss, grad_mul,
-                    dz, dstrides, accumulate, scratch):
+def distill_fwd_bwd(z, geom, strides, ids, id_strides, top, top_strides, k, weight, T, tail, reduction, loss, grad_mul, dz, dstrides,
+                    accumulate, ws, at):
     assert dz.dtype == z.dtype
+    acc, scratch, stats = _work(ws, at)
     _ck(lib.semseg_distill_fwd_bwd(_p(z), TYPES[z.dtype], *geom, *strides,
-                                   *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), _p(stats), _p(acc2),
-                                   _p(loss), float(grad_mul), _p(dz), *dstrides, int(accumulate), _p(scratch),
-                                   scratch.numel() * scratch.element_size(), _stream()), "distill_fwd_bwd")
+                                   *_teacher(ids, id_strides, top, top_strides, k, weight, T, tail, reduction), stats, acc, _p(loss),
+                                   float(grad_mul), _p(dz), *dstrides, int(accumulate), scratch,
+                                   (ws.numel() if at[2] is None else at[2]) - at[1], _stream()), "distill_fwd_bwd")
 
 
 def dropout2d_mask(mask, p, seed, offset, offset_dev=None):

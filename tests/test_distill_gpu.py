@@ -175,6 +175,13 @@ def test_labels_that_are_no_class():
     assert bool(torch.isfinite(g).all()) and float(g[1:].abs().max()) == 0
 
 
+def test_the_default_void_label_is_no_class():
+    y = torch.tensor([255, -100, 3], device=DEV)
+    few, many = (D.class_logprobs(torch.zeros(3, C, device=DEV), y) for C in (255, 256))
+    assert torch.isnan(few.logprob).tolist() == [False, True, False] and few.entropy[0] == 0
+    assert torch.isnan(many.logprob).tolist() == [False, False, False] and many.entropy[0] > 0 and many.entropy[1] == 0
+
+
 @pytest.mark.parametrize("scale", [1000.0, 1e-3])
 def test_far_and_near_logits(scale):
     gen = torch.Generator().manual_seed(8)
