@@ -85,19 +85,20 @@ struct RowTeacher {
       qrest = 0.f;
     }
   }
-  // sum of q over all entries of element i's class; what the other lanes hold comes by shuffles
-  __device__ __forceinline__ float of_class(int i, int k, int c) const {
-    float sum = 0.f;
+  // sums of q over all entries of each element's class; what the other lanes hold comes by shuffles, once for all elements
+  __device__ __forceinline__ void of_class(int k, float (&sum)[NE]) const {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) sum[i] = 0.f;
 #pragma unroll
     for (int n = 0; n < NE; ++n)
       if (n * TG < k)
         for (int src = 0; src < TG; ++src) {
           const int o = __shfl(id[n], src, TG);
           const float v = __shfl(q[n], src, TG);
-          sum += o == c ? v : 0.f;
+#pragma unroll
+          for (int i = 0; i < NE; ++i) sum[i] += o == id[i] ? v : 0.f;
           if (n * TG + src + 1 >= k) break;
         }
-    return sum;
   }
 };
 
@@ -278,12 +279,13 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(const Logits a, const
         if (!dead) {
           const float coef = g.coef(r, w), Q = rest ? q.qsum + q.qrest : q.qsum;
           const float f = coef * (rest ? Q * exp2_(lpt * LOG2E) - q.qrest : Q) / rsum;
-          float fix[NE];
+          float fix[NE], sum[NE];
+          q.of_class(t.k, sum);
 #pragma unroll
           for (int i = 0; i < NE; ++i) {
             fix[i] = 0.f;
             if (i * G < t.k) {
-              fix[i] = coef * (Q * exp2_(zj[i] * LOG2E) - q.of_class(i, t.k, q.id[i]));
+              fix[i] = coef * (Q * exp2_(zj[i] * LOG2E) - sum[i]);
               if (g.accumulate && q.id[i] >= 0) fix[i] += load1(dz + q.id[i]);
             }
           }
@@ -495,19 +497,21 @@ __global__ __launch_bounds__(256) void distill_bwd_rows_kernel(const Logits a, c
     const bool rest = t.tail && lpt != INFINITY;
     const float coef = g.coef(r, w), Q = rest ? q.qsum + q.qrest : q.qsum;
     const float off = rest ? ls + lpt : ls, f = coef * (rest ? Q * exp2_(lpt * LOG2E) - q.qrest : Q);
-    float fix[NE];
-    bool mine[NE];
+    float fix[NE], sum[NE];
+    bool mine[NE], named = false;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      fix[i] = 0.f;
       mine[i] = !dead && q.id[i] >= c0 && q.id[i] < c1 && (G < 256 || threadIdx.x < 64);
-      if (i * TG < t.k && __any(mine[i])) {      // most segments of a long row hold no entry
-        const float sum = q.of_class(i, t.k, q.id[i]);
+      named |= mine[i];
+    }
+    if (__any(named)) {                  // most segments of a long row hold no entry
+      q.of_class(t.k, sum);
+#pragma unroll
+      for (int i = 0; i < NE; ++i)
         if (mine[i]) {
-          fix[i] = coef * (Q * exp2_(((load1(z + q.id[i]) - base) * a.invT - ls) * LOG2E) - sum);
+          fix[i] = coef * (Q * exp2_(((load1(z + q.id[i]) - base) * a.invT - ls) * LOG2E) - sum[i]);
           if (g.accumulate) fix[i] += load1(dz + q.id[i]);
         }
-      }
     }
     if (G == 256) __syncthreads();       // with accumulate: the entries' old values are read before the row is written
     if (dead) {
@@ -871,7 +875,9 @@ void distill_rows_t(const Logits& a, const Teacher& t, const DistillOut& o, cons
   const int chunks = (a.C + VEC<E> - 1) / VEC<E>;
 #define DROWS(G, NV, NE) distill_rows_kernel<E, G, NV, NE, GRAD, TAIL><<<blocks, 256, 0, stream>>>(a, t, o, g)
   constexpr bool W4 = VEC<E> == 4;
-#define DROWS8(NV) do { if (t.k <= 8) DROWS(8, NV, 1); else DROWS(8, NV, 8); } while (0)
+  // entries per lane: one, two or eight, each at the cost of all it could hold (57600 x 150 fp32, k 9: 21 us with two, 29 with eight; 64
+  // lanes with an entry each 47)
+#define DROWS8(NV) do { if (t.k <= 8) DROWS(8, NV, 1); else if (t.k <= 16) DROWS(8, NV, 2); else DROWS(8, NV, 8); } while (0)
   if (chunks <= 8) DROWS8(1);
   else if (chunks <= 16) DROWS8(2);
   else if (chunks <= 24) DROWS8(3);
@@ -955,6 +961,7 @@ void distill_bwd(const Logits& a, const Teacher& t, const DistillGrad& g, hipStr
     return;
   }
   if (a.C <= 256 && t.k <= 8) distill_bwd_rows_kernel<E, 8, 1><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, t, g);
+  else if (a.C <= 256 && t.k <= 16) distill_bwd_rows_kernel<E, 8, 2><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, t, g);
   else if (a.C <= 256) distill_bwd_rows_kernel<E, 8, 8><<<dim3(1, capped((a.R + 31) / 32, 65535)), 256, 0, stream>>>(a, t, g);
   else if (a.C <= 4 * 64 * VEC<E>) distill_bwd_rows_kernel<E, 64, 1><<<dim3(1, capped((a.R + 3) / 4, 65535)), 256, 0, stream>>>(a, t, g);
   else distill_bwd_rows_kernel<E, 256, 1><<<seg_grid(a.R, a.C, 4 * 256 * VEC<E>), 256, 0, stream>>>(a, t, g);

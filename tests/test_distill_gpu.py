@@ -258,6 +258,21 @@ def test_distill(case, dt):
         check_distill(z, dim, ids, top, T, tail, weight, red, how)
 
 
+@pytest.mark.parametrize("k", [9, 15, 16, 17, 40])
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("how", ["autograd", "fused"])
+def test_distill_entries_drawn_with_repeats(k, tail, how):
+    """Entries sampled with repetition, some absent: every class collects what all its entries hold, however many a lane has."""
+    gen = torch.Generator().manual_seed(13)
+    for case, dt in ((("rows", (45,), 150, 256), torch.float32), (("rows", (45,), 21, 0), torch.bfloat16), (("rows", (5,), 700, 0), torch.float32),
+                     (("rows", (3,), 2500, 0), torch.bfloat16), (("planes", (1, 7, 5), 21, 0), torch.float32)):
+        z, dim = make(case, dt, gen)
+        ids = torch.randint(0, case[2] // 3, case[1] + (k,), generator=gen).int()
+        ids[torch.rand(ids.shape, generator=gen) < 0.1] = -1
+        top = torch.randn(ids.shape, generator=gen).double().log_softmax(-1).float() - 0.5
+        check_distill(z, dim, ids.movedim(-1, dim).to(DEV), top.movedim(-1, dim).to(DEV), 1.5, tail, None, "mean", how)
+
+
 @pytest.mark.parametrize("case", [("rows", (12,), 19, 0), ("rows", (12,), 150, 106), ("rows", (12,), 4000, 0), ("planes", (1, 4, 3), 21, 0), ("planes", (1, 4, 3), 150, 0)])
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("how", ["autograd", "fused"])
