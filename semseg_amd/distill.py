@@ -76,11 +76,11 @@ class Geom:
         self.geom = (self.n, self.p, self.C)
 
     def empty(self, size, dtype, device):
-        """A dense tensor with `size` in the place of the classes, its rows laid out like the logits'."""
-        if self.by_rows:
-            t = torch.empty(self.shape + (size,), dtype=dtype, device=device)
-            return t if self.dim == len(self.shape) else t.movedim(-1, self.dim)
-        return torch.empty(self.shape[:self.dim] + (size,) + self.shape[self.dim:], dtype=dtype, device=device)
+        """A dense tensor with `size` in the place of the classes; in memory that dimension stands behind the rows, or (planes) between
+        the n and the p of them, wherever `dim` has it."""
+        at = len(self.shape) if self.by_rows else self.outer
+        t = torch.empty(self.shape[:at] + (size,) + self.shape[at:], dtype=dtype, device=device)
+        return t if at == self.dim else t.movedim(at, self.dim)
 
     def dense(self, size):
         """Strides (sn, sp, s of `dim`) of what empty(size) gives."""
@@ -185,7 +185,8 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=Non
     with their log probabilities (falling, equal logits by rising class).  logprob, entropy and lse carry gradients.
 
     label: int64, the logits' shape without the classes.  Rows labelled ignore_index (default: 255, as in the segmentation losses, where
-    that is no class, otherwise -100) are void: not read, zero outputs, no alternatives (ids -1, log probabilities -inf), zero gradient.  A label that is neither gives log probability NaN (ops.label_check counts them).
+    that is no class, otherwise -100) are void: not read, zero outputs, no alternatives (ids -1, log probabilities -inf), zero gradient.
+    A label that is neither gives log probability NaN (ops.label_check counts them).
     A row of -inf logits has log probabilities -inf, entropy 0 and no gradient."""
     g = _check_logits(logits, class_dim, temperature)
     if label is not None:
@@ -231,7 +232,7 @@ def check_top(g, device, top_ids, top_values, weight):
     for t in (top_ids, top_values):
         s = g.strides_of(t)
         if s is None:
-            t = t.contiguous()
+            t = g.empty(k, t.dtype, device).copy_(t)
             s = g.strides_of(t)
         out += [t, s]
     return (*out, k, weight)

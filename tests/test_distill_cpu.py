@@ -39,6 +39,49 @@ def test_rows_of_a_tensor(make, dim, geom, strides, by_rows):
     assert torch.equal((i * s[0] + j * s[1] + c * s[2]).reshape(-1, 3), ei)
 
 
+LAYOUTS = {
+    "planes": lambda: (torch.zeros(2, 5, 3, 4), 1),
+    "channels_last": lambda: (torch.zeros(2, 3, 4, 5).movedim(-1, 1), 1),
+    "planes, classes named last": lambda: (torch.zeros(2, 5, 3, 4).movedim(1, -1), -1),
+    "a plane per class over the batch": lambda: (torch.zeros(5, 2, 3, 4).transpose(0, 1), 1),
+    "the same, classes named last": lambda: (torch.zeros(5, 2, 3, 4).movedim(0, -1), -1),
+    "transposed rows": lambda: (torch.zeros(5, 7).t(), 1),
+    "transposed rows of a batch": lambda: (torch.zeros(2, 5, 7).transpose(1, 2), -1),
+    "images of a larger channels_last batch": lambda: (torch.zeros(4, 3, 4, 5)[::2].movedim(-1, 1), 1),
+    "one class": lambda: (torch.zeros(2, 1, 3, 4), 1),
+    "three dimensions of pixels": lambda: (torch.zeros(2, 5, 2, 3, 4), 1),
+    "one pixel": lambda: (torch.zeros(2, 5, 1, 1), 1),
+}
+
+
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_new_tensors_lie_as_the_kernels_are_told(layout):
+    """Outputs, gradients (empty with the strides of dense) and a teacher's entries in any order of memory: row r, entry j of the tensor
+    is where the strides handed to the kernels say."""
+    z, dim = LAYOUTS[layout]()
+    dim = D._dim(z, dim)
+    g = D.Geom(z, dim)
+    rows, j = torch.arange(g.n * g.p)[:, None], torch.arange(3)
+
+    def where(s):
+        return rows // g.p * s[0] + rows % g.p * s[1] + j * s[2]
+    e = g.empty(3, torch.float32, "cpu")
+    assert e.shape == z.shape[:dim] + (3,) + z.shape[dim + 1:]
+    flat = torch.arange(e.numel())
+    assert torch.equal(where(g.dense(3)), flat.as_strided(e.shape, e.stride()).movedim(dim, -1).reshape(-1, 3))
+    d = g.dense(3)
+    assert d[2] == 1 if g.by_rows else d[1] == 1          # a gradient in the form of its logits
+    ids = torch.arange(e.numel()).view(e.shape)                # contiguous, and in two other orders
+    for t in (ids, ids.movedim(dim, -1).contiguous().movedim(-1, dim), ids.movedim(0, -1).contiguous().movedim(-1, 0)):
+        got, s, top, s2, k, _ = D.check_top(g, z.device, t, t.float(), None)
+        assert k == 3 and torch.equal(got, ids)
+        for u, us in ((got, s), (top.long(), s2)):
+            mem = torch.empty(u.numel(), dtype=torch.long)
+            mem.as_strided(u.shape, got.stride()).copy_(u)
+            assert us == s and torch.equal(mem[where(us)], ids.movedim(dim, -1).reshape(-1, 3))
+
+
+
 def test_refusals():
     z = torch.zeros(2, 5, 4, 3)
     y = torch.zeros(2, 4, 3, dtype=torch.int64)

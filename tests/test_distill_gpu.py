@@ -341,6 +341,33 @@ def test_a_student_equal_to_its_teacher_has_no_loss_and_no_gradient_on_the_entri
 # ---------------------------------------------------------------------------------------------
 # layouts, accumulation, streams, graphs
 # ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("order", [(0, 1, 2, 3), (0, 2, 3, 1), (1, 0, 2, 3)])
+@pytest.mark.parametrize("class_dim", [1, -1])
+def test_every_order_of_memory(order, class_dim, dt):
+    """Logits in each order of memory, the classes named as dimension 1 or the last, a teacher in every other order."""
+    gen = torch.Generator().manual_seed(14)
+    z = (torch.randn(3, 21, 5, 7, generator=gen) * 2).to(dt)
+    inverse = tuple(sorted(range(4), key=lambda i: order[i]))
+    v = z.to(DEV).permute(order).contiguous().permute(inverse)
+    assert torch.equal(v.cpu(), z)
+    seen = lambda t: t if class_dim == 1 else t.movedim(1, -1)  # noqa: E731
+    v = seen(v)
+    top, ids = torch.randn(3, 21, 5, 7, generator=gen).topk(4, 1)
+    for o in ((0, 1, 2, 3), (0, 2, 3, 1), (1, 0, 2, 3), (2, 0, 1, 3)):
+        back = tuple(sorted(range(4), key=lambda i: o[i]))
+        t_ids, t_top = (seen(t.to(DEV).permute(o).contiguous().permute(back)) for t in (ids, top))
+        for how in ("autograd", "fused"):
+            check_distill(v, class_dim, t_ids, t_top, 2.0, False, None, "mean", how)
+    y = labels((3, 5, 7), 21, gen, ignore=-1)
+    check_logprobs(v, class_dim, y, 1.0, 6, -1)
+    x, g1 = v.detach().requires_grad_(), torch.randn(3, 5, 7, generator=gen)
+    o = D.class_logprobs(x, y, ignore_index=-1, class_dim=class_dim)
+    grad, = torch.autograd.grad(o.logprob, x, g1.to(DEV))
+    want, b = ref.logprobs_grad(last(v, class_dim), y.cpu(), 1.0, -1, g1.double(), None, None, HALF[dt])
+    close(last(grad, class_dim), want, b, "gradient", TINY[dt])
+
+
 def test_layouts_agree_and_gradients_reach_views():
     """The same logits as planes, channels_last, pixel-major with padding, and broadcast over a batch."""
     gen = torch.Generator().manual_seed(13)
