@@ -145,8 +145,11 @@ class Trainer:
                          float(self.distill_weight))
             sig = (tuple(ids.shape), ids.dtype, values.dtype, weight is None) + e.teacher[1:]
             e.distill_buffers()
-        if sig != e._teacher_sig:         # what a recorded step bakes in of it (_host_signature)
-            e._teacher_sig, e._plan_candidate, e._plan_top = sig, None, None
+        if sig != e._teacher_sig:         # a recorded step bakes it in, and reads the buffers that go with it
+            if e._plan is not None:
+                self.plan_log.append("discarded: another form of the teacher's top classes, or none")
+            e._teacher_sig = sig
+            e._plan = e._plan_candidate = e._plan_top = None
 
     def step(self, x, y, lr=None, top=None):
         """x [N,3,H,W] fp32 cuda, y [N,h,w] int64 cuda (per-rank shard).  Returns (pred, main, aux).

@@ -715,3 +715,28 @@ def test_replayed_distillation_steps_equal_eager_ones(report):
         out = tr.step(x, y, 0.01)
     assert e._plan is not None and len(out) == 3
     assert len(tr.step(x, y, 0.01, top=(o.top_ids, o.top_logprobs))) == 4 and e._plan is None
+
+
+def test_a_record_with_a_teacher_ends_with_its_buffers():
+    """A step without a teacher that is not replayed itself ends the record of the steps with one: the next of those reads its own entries."""
+    from semseg_amd.trainer import Trainer
+    t, m = _net(77).eval(), _net(1234, dropout=0.0).train()
+    tr = Trainer(m, sync_bn=False, distill_temperature=2.0)
+    gen = torch.Generator().manual_seed(4)
+    x, y = torch.randn(2, 3, 73, 73, generator=gen).cuda(), torch.randint(0, 21, (2, 73, 73), generator=gen).cuda()
+    o = t.top_logits(x, 4)
+    for _ in range(7):
+        tr.step(x, y, 0.0, top=(o.top_ids, o.top_logprobs))
+    e = tr.engine(x)
+    assert e._plan is not None, tr.plan_log
+    tr.use_plan = False
+    tr.step(x, y, 0.0)
+    assert e._plan is None
+    tr.use_plan = True
+    for it in range(6):                  # launch by launch, recorded, replayed: the teacher's answer changes every time
+        top = (o.top_ids.roll(it, 0), o.top_logprobs.roll(it, 0) - 0.1 * it)
+        kd = tr.step(x, y, 0.0, top=top)[3]
+        s = e._rec_main["scores"]
+        want = D.distill_loss(s.data[..., :s.C].movedim(-1, 1), *top, temperature=2.0)
+        assert abs(float(kd) - float(want)) <= 1e-5 * abs(float(want)), (it, float(kd), float(want))
+    assert e._plan is not None, tr.plan_log
