@@ -306,7 +306,8 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
  * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
  * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
  * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes) aligned to 8, nothing needs to be cleared.
- * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (its alternatives: NaN and +inf first, by class).
+ * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (its alternatives: NaN first, then +inf, each by rising
+ * class).
  * semseg_class_logprobs_bwd: dz (=|+=) the gradient from those of logprob, entropy, lse (each may be NULL); 0 for rows that are void
  * or hold only -inf; strides dn, dp, dc; dz has the logits' type, one rounding. */
 enum { SEMSEG_TYPE_F32 = 0, SEMSEG_TYPE_BF16 = 1, SEMSEG_TYPE_F16 = 2 };

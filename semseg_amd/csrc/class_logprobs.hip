@@ -71,7 +71,7 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
         const unsigned long long key = pair_key(load1(z + c * a.sc), c);
         if (key < prev && key > best) best = key;
       }
-      prev = wave_max64(best);
+      prev = group_max64<64>(best);
       if (lane == 0) {
         const int c = (int)~(unsigned)prev;
         o.top_ids[ot + j * o.tk] = c;
@@ -134,16 +134,27 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
     const float ls = log2_(s) * LN2;
     if (l == 0) finish_row(o, r, a, base, s, u, ls, is_class, zy);
     if (!TOP) continue;
-    // NaN is no candidate to the maxima below: it marks what is no class of this lane and what has been taken.  A NaN of the row itself
-    // counts as +inf (every log probability of its row is NaN).
+    if (s != s) {                                  // a NaN or +inf: the alternatives one by one, NaN above +inf
+      unsigned long long prev = ~0ull;
+      for (int j = 0; j < o.k; ++j) {
+        unsigned long long best = 0;
+        for (int c = l; c < a.C; c += G) {
+          const unsigned long long key = pair_key(load1(z + c), c);
+          if (key < prev && key > best) best = key;
+        }
+        prev = group_max64<G>(best);
+        if (l == 0) {
+          o.top_ids[ot + j * o.tk] = (int)~(unsigned)prev;
+          o.top_lp[ot + j * o.tk] = s;
+        }
+      }
+      continue;
+    }
+    // NaN is no candidate to the maxima below: it marks what is no class of this lane and what has been taken.
     float cm[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int first = (i * G + l) * V;
-      if (s != s) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[i][e] = x[i][e] != x[i][e] ? INFINITY : x[i][e];
-      }
       if (first + V > a.C) {
 #pragma unroll
         for (int e = 0; e < V; ++e) x[i][e] = b[i] + e >= first && b[i] + e < a.C ? x[i][e] : NAN;
@@ -379,7 +390,7 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
         const unsigned long long key = pair_key(load1(z + c), c);
         if (key < prev && key > top) top = key;
       }
-      top = wave_max64(top);
+      top = group_max64<64>(top);
       __syncthreads();
       if (lane == 0) red64[wv] = top;
       __syncthreads();
@@ -446,7 +457,7 @@ __global__ __launch_bounds__(64) void logprobs_join_kernel(const Logits a, const
   }
   int at = 0;
   for (int j = 0; j < o.k; ++j) {
-    const unsigned long long top = wave_max64(head);
+    const unsigned long long top = group_max64<64>(head);
     if (head == top) {
       ++at;
       head = at < o.k ? lists[at * 64 + lane] : 0;

@@ -63,9 +63,10 @@ template <int G> __device__ __forceinline__ float group_sum(float v) { return gr
 template <int G> __device__ __forceinline__ unsigned group_umax(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a > b ? a : b; }); }
 template <int G> __device__ __forceinline__ unsigned group_umin(unsigned v) { return group_reduce<G>(v, [](unsigned a, unsigned b) { return a < b ? a : b; }); }
 // by two reductions: the high words, then the low words of those that have the highest
-__device__ __forceinline__ unsigned long long wave_max64(unsigned long long v) {
-  const unsigned hi = group_umax<64>((unsigned)(v >> 32));
-  const unsigned lo = group_umax<64>((unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
+template <int G>
+__device__ __forceinline__ unsigned long long group_max64(unsigned long long v) {
+  const unsigned hi = group_umax<G>((unsigned)(v >> 32));
+  const unsigned lo = group_umax<G>((unsigned)(v >> 32) == hi ? (unsigned)v : 0u);
   return (unsigned long long)hi << 32 | lo;
 }
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
