@@ -53,14 +53,14 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
     for (int c = lane; c < a.C; c += 64) m = fmaxf(m, load1(z + c * a.sc));
     m = group_max<64>(m);
     const float base = m == -INFINITY ? 0.f : m;
-    float s = 0.f, u = 0.f;
+    float s = 0.f, u = 0.f, lost_s = 0.f, lost_u = 0.f;
     for (int c = lane; c < a.C; c += 64) {
       const float d = (load1(z + c * a.sc) - base) * a.scale2, e = exp2_(d);
-      s += e;
-      u += e * fmaxf(d, -300.f);               // exp2(-300) = 0 in fp32; 0 * -inf would be NaN
+      add_group(s, lost_s, e);
+      add_group(u, lost_u, e * fmaxf(d, -300.f));      // exp2(-300) = 0 in fp32; 0 * -inf would be NaN
     }
-    s = group_sum<64>(s);
-    u = group_sum<64>(u);
+    s = at_least_one(group_sum<64>(s));
+    u = not_positive(group_sum<64>(u));
     const float ls = log2_(s) * LN2;
     const bool is_class = y >= 0 && y < a.C;
     if (lane == 0) finish_row(o, r, a, base, s, u, ls, is_class, o.logprob && is_class ? load1(z + y * a.sc) : 0.f);
@@ -252,7 +252,8 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
   const E* z = (const E*)a.z + a.at(r);
   const int c0 = sp * t.slice, c1 = min(a.C, c0 + t.slice);
   const int iters = (c1 - c0 + 256 * V - 1) / (256 * V);
-  float m = -INFINITY, s = 0.f, u = 0.f, lm = -INFINITY;
+  RowSums sum;
+  float lm = -INFINITY;
   constexpr int UN = 4;
   for (int it = 0; it < iters; it += UN) {
     float x[UN][V], cm[UN];
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
         }
       }
     }
-    float nm = m;
+    float nm = sum.m;
 #pragma unroll
     for (int n = 0; n < UN; ++n) {
       cm[n] = x[n][0];
@@ -283,35 +284,33 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         lm = fmaxf(lm, group_max<8>(cm[n]));
-        const int q = it + n;
-        if (q < iters && ((q + 1) % t.join == 0 || q + 1 == iters)) {
-          if ((tid & 7) == 0) line[(q / t.join) * 32 + g8] = order_key(lm);
+        const int i = it + n;
+        if (i < iters && ((i + 1) % t.join == 0 || i + 1 == iters)) {
+          if ((tid & 7) == 0) line[(i / t.join) * 32 + g8] = order_key(lm);
           lm = -INFINITY;
         }
       }
     }
-    const float base = nm == -INFINITY ? 0.f : nm;
-    rescale(s, u, m, base, a.scale2);
-    m = nm;
+    const float base = sum.follow(nm, a.scale2);
+    float gs = 0.f, gu = 0.f;
 #pragma unroll
     for (int n = 0; n < UN; ++n)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = (x[n][e] - base) * a.scale2, w = exp2_(d);
-        s += w;
-        u += w * fmaxf(d, -300.f);
+        gs += w;
+        gu += w * fmaxf(d, -300.f);
       }
+    sum.add(gs, gu);
   }
   // join the lanes, then the waves
-  const float wm = group_max<64>(m);
-  rescale(s, u, m, wm == -INFINITY ? 0.f : wm, a.scale2);
-  s = group_sum<64>(s);
-  u = group_sum<64>(u);
+  const float wm = group_max<64>(sum.m);
+  sum.settle(wm, a.scale2);
+  float s = group_sum<64>(sum.s), u = group_sum<64>(sum.u);
   if (lane == 0) { red[0][wv] = wm; red[1][wv] = s; red[2][wv] = u; }
   if (tid == 0) nlines = ncand = 0;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float base = m == -INFINITY ? 0.f : m;
+  const float m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3])), base = usable(m);
   s = u = 0.f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -320,6 +319,8 @@ __global__ __launch_bounds__(256) void logprobs_stream_kernel(const Logits a, co
     s += sw;
     u += uw;
   }
+  s = at_least_one(s);
+  u = not_positive(u);
   const float ls = log2_(s) * LN2;
   if (tid == 0) {
     if (t.nsplit > 1) {
@@ -534,13 +535,13 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   const unsigned bytes = px.template bytes<E>();
   const E* z = zt + (px.px - px.base);
   const int per = (a.C + SPLIT - 1) / SPLIT, c0 = wv * per, c1 = min(a.C, c0 + per);
-  float m[PV], s[PV], u[PV], zy[PV];
+  RowSums sum[PV];
+  float zy[PV];
   int yc[PV];
   B best[PV];
 #pragma unroll
   for (int v = 0; v < PV; ++v) {
-    m[v] = -INFINITY;
-    s[v] = u[v] = zy[v] = 0.f;
+    zy[v] = 0.f;
     if (ZY) {
       const long long y = o.logprob ? o.label[i * a.p + px.px + v] : -1;
       yc[v] = y >= 0 && y < a.C ? (int)y : -1;
@@ -566,18 +567,18 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
     }
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
-      float nm = m[v];
+      float nm = sum[v].m;
 #pragma unroll
       for (int n = 0; n < UN; ++n) nm = fmaxf(nm, x[n][v]);
-      const float base = nm == -INFINITY ? 0.f : nm;
-      rescale(s[v], u[v], m[v], base, a.scale2);
-      m[v] = nm;
+      const float base = sum[v].follow(nm, a.scale2);
+      float gs = 0.f, gu = 0.f;
 #pragma unroll
       for (int n = 0; n < UN; ++n) {
         const float d = (x[n][v] - base) * a.scale2, w = exp2_(d);
-        s[v] += w;
-        u[v] += w * fmaxf(d, -300.f);
+        gs += w;
+        gu += w * fmaxf(d, -300.f);
       }
+      sum[v].add(gs, gu);
     }
     if (ZY) {
 #pragma unroll
@@ -602,6 +603,14 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
     if (c + UN >= c1) break;
     if (c + 2 * UN < c1) load(qa, c + 2 * UN);
     work(qb, c + UN);
+  }
+  float m[PV], s[PV], u[PV];
+#pragma unroll
+  for (int v = 0; v < PV; ++v) {
+    sum[v].settle(sum[v].m, a.scale2);
+    m[v] = sum[v].m;
+    s[v] = sum[v].s;
+    u[v] = sum[v].u;
   }
   if constexpr (SPLIT > 1) {
     if (wv > 0) {
@@ -653,7 +662,9 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
     y[v] = o.label ? o.label[r + v] : 0;
     empty[v] = o.label && y[v] == o.ignore;
     is_class[v] = y[v] >= 0 && y[v] < a.C;
-    base[v] = m[v] == -INFINITY ? 0.f : m[v];
+    base[v] = usable(m[v]);
+    s[v] = at_least_one(s[v]);
+    u[v] = not_positive(u[v]);
     ls[v] = log2_(s[v]) * LN2;
   }
   if (o.logprob) {

@@ -191,6 +191,47 @@ __device__ __forceinline__ void rescale(float& s, float& u, float from, float to
   s = s * f;
 }
 
+// ---- sums over thousands of classes.  Equal terms that are added to a large sum one by one round the same way every time (65536 classes of
+// two values: 1.3e-4 of log S), and so does a sum that is moved to a new base with every small rise of the maximum.  So a group of 8 to 32
+// terms is added up by itself, the groups with what the last addition rounded away (`lost`) taken along, and the base of running sums follows
+// the maximum only once the sum is to be halved at least: older moves fade with what they moved.
+__device__ __forceinline__ void add_group(float& s, float& lost, float g) {
+  const float y = g - lost, t = s + y;
+  lost = (t - s) - y;
+  s = t;
+}
+// `base` -inf: nothing to move yet
+__device__ __forceinline__ bool must_move(float top, float base, float scale2) { return (top - base) * scale2 >= 1.f; }
+__device__ __forceinline__ float usable(float base) { return base == -INFINITY ? 0.f : base; }
+// A sum about the row's maximum holds a term 1: where its last move has rounded it below that, no probability gets above 1.  (NaN stays.)
+__device__ __forceinline__ float at_least_one(float s) { return s > 0.f && s < 1.f ? 1.f : s; }
+__device__ __forceinline__ float not_positive(float u) { return u > 0.f ? 0.f : u; }
+
+// Running sums of e^d (s) and of e^d d (u) of one lane; d in units of log 2
+struct RowSums {
+  float m = -INFINITY, base = -INFINITY, s = 0.f, u = 0.f, lost_s = 0.f, lost_u = 0.f;      // m: the maximum so far
+  // the maximum has become `top`: the base to take d about
+  __device__ __forceinline__ float follow(float top, float scale2) {
+    m = top;
+    const bool mv = must_move(top, base, scale2);
+    if (__any(mv)) {
+      const float to = mv ? top : base, d = (base - usable(to)) * scale2, f = exp2_(d);
+      u = (u + s * fmaxf(d, -300.f)) * f;
+      s *= f;
+      lost_u = (lost_u + lost_s * fmaxf(d, -300.f)) * f;
+      lost_s *= f;
+      base = to;
+    }
+    return usable(base);
+  }
+  __device__ __forceinline__ void add(float gs, float gu) {
+    add_group(s, lost_s, gs);
+    add_group(u, lost_u, gu);
+  }
+  // about the maximum itself (or a larger one)
+  __device__ __forceinline__ void settle(float to, float scale2) { rescale(s, u, base, usable(to), scale2); }
+};
+
 // ---- planes: PV neighbouring pixels to a lane, classes in a loop; every load of a wave is one contiguous piece of a class's plane.
 // Where planes are written, or a tile is a single wave, neighbouring tiles go to the same XCD (xcd_remap), so that what runs there at a
 // time walks through one piece of every plane (the distillation gradient of 4 x 150 x 473 x 473: 229 us, with tiles dealt out in turn 265).

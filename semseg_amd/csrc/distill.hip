@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, con
     id = c >= 0 && c < a.C ? (int)c : -1;
   }
   const int first = sp * d.slice, last = min(a.C, first + d.slice);
-  float m = -INFINITY, s = 0.f, unused = 0.f;
+  float m = -INFINITY, b = -INFINITY, s = 0.f, lost = 0.f;      // maximum, base of the sum, sum, what it lost
   constexpr int TURN = TAIL ? MAP_CHUNKS * V : 1 << 30;
   for (int c0 = first; c0 < last; c0 += TURN) {
     const int c1 = last - c0 > TURN ? c0 + TURN : last;
@@ -394,18 +394,25 @@ __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, con
       for (int n = 0; n < UN; ++n)
 #pragma unroll
         for (int e = 0; e < V; ++e) nm = fmaxf(nm, x[n][e]);
-      const float base = nm == -INFINITY ? 0.f : nm;
-      s *= exp2_((m - base) * a.scale2);
       m = nm;
+      const bool mv = must_move(m, b, a.scale2);
+      if (__any(mv)) {
+        const float to = mv ? m : b, f = exp2_((b - usable(to)) * a.scale2);
+        s *= f;
+        lost *= f;
+        b = to;
+      }
+      const float base = usable(b);
+      float gs = 0.f;
 #pragma unroll
       for (int n = 0; n < UN; ++n)
 #pragma unroll
-        for (int e = 0; e < V; ++e) s += exp2_((x[n][e] - base) * a.scale2);
+        for (int e = 0; e < V; ++e) gs += exp2_((x[n][e] - base) * a.scale2);
+      add_group(s, lost, gs);
     }
   }
   const float wm = group_max<64>(m);
-  rescale(s, unused, m, wm == -INFINITY ? 0.f : wm, a.scale2);
-  s = group_sum<64>(s);
+  s = group_sum<64>(s * exp2_((b - usable(wm)) * a.scale2));
   if ((tid & 63) == 0) { red[0][tid >> 6] = wm; red[1][tid >> 6] = s; }
   __syncthreads();
   if (tid == 0) {
@@ -453,7 +460,7 @@ __global__ __launch_bounds__(256) void distill_join_kernel(const Logits a, const
     const float base = m == -INFINITY ? 0.f : m;
     s *= exp2_((m1 - base) * a.scale2);
     if (t.tail && once) s += exp2_((zj - base) * a.scale2);
-    s = group_sum<64>(s);
+    s = at_least_one(group_sum<64>(s));
     const float ls = log2_(s) * LN2;
     const float lp = s == 0.f ? -INFINITY : (zj - base) * a.invT - ls;
     float kl = group_sum<64>(q.q[0] == 0.f ? 0.f : q.q[0] * (q.lq[0] - lp));
@@ -656,14 +663,30 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
     const unsigned bytes = px.template bytes<E>();
     const E* z = zt + (px.px - px.base);
     const long long r0 = i * a.p + px.px, io = i * t.in + px.px * t.ip, vo = i * t.vn + px.px * t.vp;
-    float m[PV], base[PV], s[PV], st[PV], dot[PV], qacc[PV];
+    // maximum, base, sums about it and what they lost: all classes, those outside the entries, q (z - base) of the entries; q so far
+    float m[PV], base[PV], s[PV], st[PV], dot[PV], lost_s[PV], lost_t[PV], lost_d[PV], qacc[PV];
     PixTeacher<KR> q[PV];
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
       q[v].init(t, a, io + v * t.ip, vo + v * t.vp);
-      m[v] = -INFINITY;
-      base[v] = s[v] = st[v] = dot[v] = qacc[v] = 0.f;
+      m[v] = base[v] = -INFINITY;
+      s[v] = st[v] = dot[v] = lost_s[v] = lost_t[v] = lost_d[v] = qacc[v] = 0.f;
     }
+    // everything of pixel v about the base `to`
+    const auto move = [&](int v, float to) {
+      const float f = exp2_((base[v] - usable(to)) * a.scale2);
+      s[v] *= f;
+      lost_s[v] *= f;
+      if (TAIL) {
+        st[v] *= f;
+        lost_t[v] *= f;
+      }
+      if (qacc[v] != 0.f) {
+        add_group(dot[v], lost_d[v], qacc[v] * (usable(base[v]) - usable(to)));
+        if (!(fabsf(dot[v]) < INFINITY)) lost_d[v] = 0.f;      // an entry on a class of -inf: -inf stays
+      }
+      base[v] = to;
+    };
     for (int c0 = c_lo; c0 < c_hi; c0 += CH) {
       E x[CH][PV];
 #pragma unroll
@@ -677,25 +700,31 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
           nm = fmaxf(nm, y[n]);
           tile[n][lane * PV + v] = y[n];
         }
-        const float nb = nm == -INFINITY ? 0.f : nm, f = exp2_((m[v] - nb) * a.scale2);
-        s[v] *= f;
-        if (TAIL) st[v] *= f;
-        dot[v] += qacc[v] == 0.f ? 0.f : qacc[v] * (base[v] - nb);
         m[v] = nm;
-        base[v] = nb;
+        const bool mv = must_move(nm, base[v], a.scale2);
+        if (__any(mv)) move(v, mv ? nm : base[v]);
+        const float nb = usable(base[v]);
         unsigned in = 0;
         q[v].in_chunk(t, a, io + v * t.ip, vo + v * t.vp, c0, [&](int n, float qc) {
           in |= 1u << n;
           dot[v] += qc == 0.f ? 0.f : qc * (tile[n][lane * PV + v] - nb);
           qacc[v] += qc;
         });
+        float gs = 0.f, gt = 0.f;
 #pragma unroll
         for (int n = 0; n < CH; ++n) {
           const float p = exp2_((y[n] - nb) * a.scale2);
-          s[v] += p;
-          if (TAIL) st[v] += in >> n & 1u ? 0.f : p;
+          gs += p;
+          if (TAIL) gt += in >> n & 1u ? 0.f : p;
         }
+        add_group(s[v], lost_s[v], gs);
+        if (TAIL) add_group(st[v], lost_t[v], gt);
       }
+    }
+#pragma unroll
+    for (int v = 0; v < PV; ++v) {
+      move(v, m[v]);
+      base[v] = usable(m[v]);
     }
     if constexpr (SPLIT > 1) {
       __syncthreads();                 // the tile before this one has been joined
@@ -733,21 +762,26 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
 #pragma unroll
     for (int v = 0; v < PV; ++v) {
       const float w = t.weight ? t.weight[r0 + v] : 1.f;
+      s[v] = at_least_one(s[v]);
       const float ls = log2_(s[v]) * LN2;
       float lpt = 0.f, kl = s[v] == 0.f ? (q[v].qsum > 0.f ? INFINITY : 0.f) : q[v].qlogq - (dot[v] * a.invT - q[v].qsum * ls);
       bool rest = TAIL;
       if (TAIL) {
         lpt = log2_(st[v]) * LN2 - ls;
         if (st[v] < 1e-20f) {          // the rest is far below the row's maximum: once more, about its own
-          float mt = -INFINITY, sum = 0.f;
+          float mt = -INFINITY, sum = 0.f, lost = 0.f;
           for (int c = 0; c < a.C; ++c) {
             const float y = load1(z + c * a.sc + v);
             bool in = false;
             for (int j = 0; j < t.k; ++j) in |= t.id(io + v * t.ip, j) == c;
             if (in || y == -INFINITY) continue;
-            const float nm = fmaxf(mt, y);
-            sum = sum * exp2_((mt - nm) * a.scale2) + exp2_((y - nm) * a.scale2);
-            mt = nm;
+            if (must_move(y, mt, a.scale2)) {
+              const float f = exp2_((mt - y) * a.scale2);
+              sum *= f;
+              lost *= f;
+              mt = y;
+            }
+            add_group(sum, lost, exp2_((y - mt) * a.scale2));
           }
           rest = mt != -INFINITY;
           lpt = rest ? (mt - base[v]) * a.invT + log2_(sum) * LN2 - ls : 0.f;
