@@ -167,6 +167,12 @@ class Trainer:
         if e.params_stale():
             raise RuntimeError("the module tree changed after the Trainer built its engine; build a new Trainer")
         self._set_teacher(e, top)
+        try:
+            return self._step(e, x, y, lr)
+        finally:
+            e.teacher = None              # this step's alone: a backward pass of the engine outside step() has none
+
+    def _step(self, e, x, y, lr):
         if not (self.use_plan and e.ktimer is None and e.tape_hook is None and not e._plan_off):
             if e._plan_replays:
                 self._set_step_state(e, lr, 0)      # the device part of the dropout counter belongs to replayed steps only
