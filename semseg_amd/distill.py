@@ -127,6 +127,30 @@ def _overlap(a, b):
     return a.device == b.device and a.numel() and b.numel() and a.data_ptr() < span(b) and b.data_ptr() < span(a)
 
 
+def _once(t):
+    """Whether no two values of a tensor share memory: every stride passes over all that the smaller ones reach."""
+    reach = 0
+    for st, n in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+        if st <= reach:
+            return False
+        reach += st * (n - 1)
+    return True
+
+
+def _check_out(out, logits, g, inputs):
+    """Strides of the tensor that a gradient is written to."""
+    if out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("out must have the logits' shape, type and device")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out must not require a gradient")
+    if any(_overlap(out, t) for t in inputs if t is not None):
+        raise ValueError("out shares memory with an input")
+    ds = g.strides_of(out)
+    if ds is None or not (ds[2] == 1 if g.by_rows and g.C > 1 else g.C == 1 or ds[1] == 1) or not _once(out):
+        raise ValueError("out of strides %s does not have the logits' layout, each value in a place of its own" % (tuple(out.stride()),))
+    return ds
+
+
 def _on_gpu(z):
     if not z.is_cuda:
         raise RuntimeError("semseg_amd runs on the MI355X only: move the logits to cuda (there is no CPU fallback)")
@@ -307,16 +331,7 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
             raise ValueError("accumulate=True needs out")
         out, ds = g.empty(g.C, logits.dtype, dev), g.dense(g.C)
     else:
-        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev:
-            raise ValueError("out must have the logits' shape, type and device")
-        if out.requires_grad and torch.is_grad_enabled():
-            raise ValueError("out must not require a gradient")
-        if any(_overlap(out, t) for t in (logits, top_ids, top_logits, weight) if t is not None):
-            raise ValueError("out shares memory with an input")
-        ds = g.strides_of(out)
-        if ds is None or not (ds[2] == 1 if g.by_rows and g.C > 1 else g.C == 1 or ds[1] == 1) or any(
-                st == 0 and n > 1 for n, st in zip(out.shape, out.stride())):
-            raise ValueError("out of strides %s does not have the logits' layout" % (tuple(out.stride()),))
+        ds = _check_out(out, logits, g, (logits, top_ids, top_logits, weight))
     with _on_device(logits):
         # rows that fit registers need no statistics kept for a second pass
         nbytes, at = ops.distill_workspace(logits.dtype, *g.geom, g.strides[2], stats=not (g.by_rows and g.C <= ops.ROW_CLASSES))
