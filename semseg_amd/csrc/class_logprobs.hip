@@ -905,10 +905,9 @@ void logprobs_fwd(const Logits& a, const LogprobOut& o, int type, void* scratch,
     else if (chunks <= 8) ROWS(4, 2);
     else if (chunks <= 12) ROWS(4, 3);
     else if (chunks <= 20) ROWS(4, 5);
-    else if (W4 && chunks <= 40) ROWS(4, W4 ? 10 : 1);
-    else if (!W4 && chunks <= 32) ROWS(8, W4 ? 1 : 4);
-    else if (W4 && chunks <= 64) ROWS(8, W4 ? 8 : 1);
-    else if (chunks <= 64) ROWS(64, 1);
+    else if (W4 && chunks <= 40) ROWS(4, W4 ? 10 : 1);           // a form that only the other type reaches names one of this type's
+    else if (chunks <= (W4 ? 64 : 32)) ROWS(8, W4 ? 8 : 4);      // 256 classes
+    else if (!W4 && chunks <= 64) ROWS(64, W4 ? 2 : 1);
     else if (chunks <= 128) ROWS(64, 2);
     else if (chunks <= 256) ROWS(64, 4);
     else ROWS(64, W4 ? 8 : 1);

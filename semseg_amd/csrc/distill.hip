@@ -917,7 +917,7 @@ void distill_rows_t(const Logits& a, const Teacher& t, const DistillOut& o, cons
   else if (chunks <= 24) DROWS8(3);
   else if (W4 && chunks <= 40) DROWS8(W4 ? 5 : 1);
   else if (chunks <= (W4 ? 64 : 32)) DROWS8(W4 ? 8 : 4);
-  else if (chunks <= 64) DROWS(64, 1, 1);
+  else if (!W4 && chunks <= 64) DROWS(64, W4 ? 2 : 1, 1);
   else if (chunks <= 128) DROWS(64, 2, 1);
   else if (chunks <= 256) DROWS(64, 4, 1);
   else DROWS(64, W4 ? 8 : 1, 1);
