@@ -303,7 +303,8 @@ int semseg_bilinear_nhwc_to_nchw(const float* x, int ldx, float* y, int N, int H
  * semseg_class_logprobs_fwd: log softmax(z / T) at the row's label (logprob; needs label), its entropy, lse = log sum exp(z / T), and
  * the k <= SEMSEG_CLASS_TOP_MAX classes of the largest logits with their log probabilities, in falling order, equal logits by rising
  * class; row (i, j)'s alternative a is element i * tn + j * tp + a * tk of top_ids / top_logprobs.  Any output may be NULL.  stats
- * [2][n * p]: for the backward call.  Rows whose label is ignore_index are not read: 0, 0, 0, ids -1, log probabilities -inf.  A label
+ * [2][n * p]: for the backward call.  Rows whose label is ignore_index are void: 0, 0, 0, ids -1, log probabilities -inf, whatever they
+ * hold (where the pixels are contiguous they are read all the same: the memory must be readable).  A label
  * that is neither ignore_index nor in [0, C): logprob NaN.  A row of -inf logits: lse and every log probability -inf, entropy 0.
  * scratch: semseg_class_logprobs_scratch_bytes() bytes (0 for most shapes) aligned to 8, nothing needs to be cleared.
  * A NaN or +inf logit makes its own row's log probabilities, entropy and lse NaN (its alternatives: NaN first, then +inf, each by rising
@@ -329,7 +330,7 @@ int semseg_class_logprobs_bwd(const void* z, int type, long long n, long long p,
  *             sides, q_rest = max(0, 1 - sum q); without a finite logit outside ids there is no such class
  * with p = softmax(z / T).  rows: T^2 * weight_r * loss_r (needed by SEMSEG_REDUCE_NONE, else may be NULL).  loss: their sum (SUM),
  * over the sum of weights (MEAN; NaN where that is 0, like an all-void cross entropy; gradients 0).  weight NULL: 1; rows of weight 0
- * are not read.  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
+ * are void: loss and gradient 0 whatever their logits, ids and values hold (read all the same where the pixels are contiguous).  An id >= C: the row's loss is NaN, its gradient 0.  stats [3][n * p], acc2 [2]: for the backward call.  scratch:
  * semseg_distill_scratch_bytes() bytes aligned to 8, nothing needs to be cleared; no atomics, results do not depend on scheduling.
  * _bwd: dz (=|+=) grad_mul * grad_loss (one device float, one per row for NONE, NULL: 1) * d loss / dz.
  * _fwd_bwd: loss and grad_mul * d loss / dz (MEAN or SUM) in one call; stats may be NULL for rows of contiguous classes up to

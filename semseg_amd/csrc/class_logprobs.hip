@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256) void logprobs_fwd_kernel(const Logits a, const
 // Few lanes to a row, because most of an alternative's instructions cost the same whatever they serve: with 4 lanes 16 rows a wave.
 // An alternative is one round: the lanes' chunk maxima, their largest, the lowest class that has it, that class taken out and its chunk's
 // maximum renewed.  The chunks lie in LDS too, where a lane reads the one that it needs by its number (selecting it from registers, and
-// changing it there, took twice the instructions: 57600 x 150, 8 alternatives: 22.9 us).  16.8 us now, bound by instructions (100 a row,
-// 85 % of the issue slots); its 39 MB would take 5.5.
+// changing it there, took twice the instructions: 57600 x 150, 8 alternatives: 22.9 us).  16 us now, bound by the instructions of this
+// selection (100 a row, 85 % of the issue slots); its 39 MB would take 5.5.  Each alternative is a round behind the one before: k 64 takes 56.
 template <typename E, int G, int NV, bool TOP>
 __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, const LogprobOut o) {
   constexpr int V = VEC<E>;
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(256) void logprobs_rows_kernel(const Logits a, cons
 //   tau = the k-th largest of the 256 lanes' maxima over their lines' maxima (a bound: at least k logits are >= tau),
 //   the lines whose maximum is >= tau are read again (about k of them), their logits >= tau collected and ranked by counting.
 // With many equal logits the lists could run over: then (and where a NaN hides from the maxima) the k best are taken in k passes.
-// Bound by memory: 4096 x 50001 bf16, 16 alternatives: 95 us, 4.3 TB/s (a copy reaches 4.75); one row of 131072 in 32 slices: 8 us and 7.5
+// Bound by memory: 4096 x 50001 bf16, 16 alternatives: 96 us, 4.3 TB/s (a copy reaches 4.8); one row of 131072 in 32 slices: 8 us and 7.6
 // for joining them.
 constexpr int LINES = 4096, CAND = 512, CLINES = 256;
 
@@ -512,15 +512,16 @@ constexpr int PLANE_K = 32;
 template <typename E> constexpr int PLANE_CLASSES = CLASS_BITS<E> ? (int)CLASS_BITS<E> + 1 : 65536;
 
 // One pass over a pixel's classes with a running maximum, 8 classes at a time, the lists beside it.  SPLIT = 4: a block's four waves share
-// 64 * PV pixels and take a quarter of the classes each (images too small to fill the device).  Bound by memory where classes are many:
-// 8 x 150 x 473 x 473 fp32, 3 alternatives: 223 us, 5.1 TB/s; by instructions where they are few: 2 x 19 x 713 x 713 bf16: 20 us, 4.1 TB/s.
+// 64 * PV pixels and take a quarter of the classes each (images too small to fill the device).  Bound by memory up to a few alternatives:
+// 8 x 150 x 473 x 473 fp32: 210 us without any (5.1 TB/s), 236 with 3; by the lists' instructions beyond: 334 with 8, 582 with 16, 939 with
+// 32.  2 x 19 x 713 x 713 bf16, 3 alternatives: 21 us, 3.9 TB/s, memory and instructions alike.
 template <typename E, int PV, int K, int SPLIT>
 __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, const LogprobOut o, const long long i0, const int tiles) {
   using B = Best<E, K>;
   constexpr bool IDS = B::BITS == 0 && K > 0;
   // The label's logit is kept as it comes by (fp32), or fetched afterwards (16 bits): the one costs two instructions a logit, the other a
-  // memory line a pixel.  8 x 150 x 473 x 473 fp32: 250 against 265 us; 2 x 19 x 713 x 713 bf16, whose two pixels to a lane leave no
-  // instructions to spare: 24 against 21.
+  // memory line a pixel.  8 x 150 x 473 x 473 fp32: 6 % less time than the other way; 2 x 19 x 713 x 713 bf16, whose two pixels to a lane
+  // leave no instructions to spare: 14 % more.
   constexpr bool ZY = sizeof(E) == 4;
   constexpr int LANES = 256 / SPLIT, UN = 8;
   __shared__ float red[SPLIT > 1 ? SPLIT - 1 : 1][4][PV][SPLIT > 1 ? 64 : 1];
@@ -528,7 +529,7 @@ __global__ __launch_bounds__(256) void logprobs_planes_kernel(const Logits a, co
   __shared__ int ids[SPLIT > 1 && IDS ? SPLIT - 1 : 1][K > 0 ? K : 1][PV][SPLIT > 1 && IDS ? 64 : 1];
   const int wv = SPLIT > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0, pl = threadIdx.x & (LANES - 1);
   unsigned image, at;
-  tile_of(blockIdx.x, tiles, image, at);      // reads alone, 1 KB a block: 223 us as dealt out, 230 with neighbours on one XCD
+  tile_of(blockIdx.x, tiles, image, at);      // reads alone, 1 KB a block: with neighbours on one XCD 3 % more time
   const long long i = i0 + image;
   const Px<PV> px((long long)at * (LANES * PV), pl, a.p);
   const E* zt = (const E*)a.z + i * a.sn + px.base;
@@ -755,7 +756,7 @@ struct RowGrad {
 };
 
 // Contiguous classes: G lanes to a row (8, 64) or a block to a segment of SEG chunks a lane; one read, one write, no reductions.  Bound by
-// memory: 4096 x 32000 bf16: 83 us, 6.3 TB/s (part of what the forward pass read is still in the last-level cache).
+// memory: 4096 x 32000 bf16: 84 us, 6.3 TB/s (part of what the forward pass read is still in the last-level cache).
 template <typename E, int G>
 __global__ __launch_bounds__(256) void logprobs_bwd_rows_kernel(const Logits a, const LogprobGrad g) {
   constexpr int V = VEC<E>, SEG = 4;
@@ -789,7 +790,8 @@ __global__ __launch_bounds__(256) void logprobs_bwd_rows_kernel(const Logits a, 
   }
 }
 
-// Planes: PV pixels and a slice of the classes to a lane.  Bound by memory: 4 x 21 x 473 x 473 fp32: 31 us, 4.9 TB/s.
+// Planes: PV pixels and a slice of the classes to a lane.  Bound by memory: 4 x 21 x 473 x 473 fp32: 28 us, 6.3 TB/s (part of what the
+// forward pass read is still in the last-level cache).
 template <typename E, int PV>
 __global__ __launch_bounds__(256) void logprobs_bwd_planes_kernel(const Logits a, const LogprobGrad g, const long long i0, const int tiles,
                                                                   const int slice) {

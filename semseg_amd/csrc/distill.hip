@@ -170,7 +170,7 @@ __global__ __launch_bounds__(1024) void distill_finish_kernel(const double* part
 
 // Rows of at most 2048 contiguous classes: G lanes hold a row in registers (8 up to 256 classes; 4 lanes to a row save instructions, but
 // what bounds this kernel is the way from the entries' ids to the logits gathered there, and with them fewer waves share it: 57600 x 150,
-// k 8: 26.8 us, with 8 lanes 21; with the ids fetched before the logits 19.7, where 73 MB would take 10.4).  GRAD: loss and gradient from
+// k 8: 26.8 us, with 8 lanes 21; with the ids fetched before the logits 20, where 73 MB would take 10.4; k 32: 42, k 64: 58).  GRAD: loss and gradient from
 // one read of the logits.
 template <typename E, int G, int NV, int NE, bool GRAD, bool TAIL>
 __global__ __launch_bounds__(256) void distill_rows_kernel(const Logits a, const Teacher t, const DistillOut o, const DistillGrad g) {
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(256) void distill_stream_kernel(const Logits a, con
     q[1] = s;
   }
 }
-// ... and one wave a row joins them, adds the entries' logits and takes the loss.  2048 x 131072 bf16, k 32 with a tail: 122 us (4.4 TB/s)
+// ... and one wave a row joins them, adds the entries' logits and takes the loss.  2048 x 131072 bf16, k 32 with a tail: 120 us (4.5 TB/s)
 // and 9.
 template <typename E>
 __global__ __launch_bounds__(256) void distill_join_kernel(const Logits a, const Teacher t, const DistillOut o, const DStream d) {
@@ -642,7 +642,8 @@ struct PixTeacher {
 };
 
 // Loss: S about the running maximum, the mass outside the entries about the same one, sum q d as it goes.  A wave has 64 * PV pixels;
-// with SPLIT = 4 four waves share them and take a quarter of the classes each.  4 x 150 x 473 x 473 fp32, k 4: 127 to 153 us for 537 MB.
+// with SPLIT = 4 four waves share them and take a quarter of the classes each.  4 x 150 x 473 x 473 fp32, k 4: 122 to 159 us for 537 MB; k 8:
+// 152.  Beyond 8 entries (KR = 0) they are read again with every CH classes: k 16: 562 us, k 64: 2107.
 template <typename E, int PV, int KR, int SPLIT, bool TAIL>
 __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits a, const Teacher t, const DistillOut o, const int tiles,
                                                                     const long long all) {
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(64 * SPLIT) void distill_planes_kernel(const Logits
   block_part<64 * SPLIT>(o.part, loss, wsum);
 }
 
-// 4 x 150 x 473 x 473 fp32, k 4: 229 us, 4.7 TB/s.
+// 4 x 150 x 473 x 473 fp32, k 4: 227 us, 4.7 TB/s.
 // The tile holds -coef * q; with a tail a class of the teacher is marked in the word's last bit (half a step of fp32 at most).
 template <typename E, int PV, int KR, bool TAIL>
 __global__ __launch_bounds__(64) void distill_bwd_planes_kernel(const Logits a, const Teacher t, const DistillGrad g, const long long i0,
@@ -972,7 +973,8 @@ void distill_fwd(const Logits& a, const Teacher& t, const DistillOut& o, int typ
 template <typename E>
 void distill_bwd(const Logits& a, const Teacher& t, const DistillGrad& g, hipStream_t stream) {
   if (a.C > 1 && a.sc != 1) {
-    // two pixels to a lane: 8 bytes a load and store of fp32 (4 x 150 x 473 x 473: 264 us, with one 290, with four 259 but slower on small images)
+    // two pixels to a lane: 8 bytes a load and store of fp32 (4 x 150 x 473 x 473: 10 % less time than with one; four take 2 % less still, but
+    // more on small images)
     constexpr int PV = 2;
     const int pv = a.p >= PV ? PV : 1;
     const long long tiles = (a.p + 64 * pv - 1) / (64 * pv), blocks = a.R / a.p * tiles;

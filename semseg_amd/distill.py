@@ -209,9 +209,11 @@ def class_logprobs(logits, label=None, topk=0, temperature=1.0, ignore_index=Non
     with their log probabilities (falling, equal logits by rising class).  logprob, entropy and lse carry gradients.
 
     label: int64, the logits' shape without the classes.  Rows labelled ignore_index (default: 255, as in the segmentation losses, where
-    that is no class, otherwise -100) are void: not read, zero outputs, no alternatives (ids -1, log probabilities -inf), zero gradient.
+    that is no class, otherwise -100) are void, whatever they hold: zero outputs, no alternatives (ids -1, log probabilities -inf), zero
+    gradient.
     A label that is neither gives log probability NaN (ops.label_check counts them).
-    A row of -inf logits has log probabilities -inf, entropy 0 and no gradient."""
+    A row of -inf logits has log probabilities -inf, entropy 0 and no gradient.  A row with a NaN or +inf has NaN in everything but its
+    alternatives: NaN first, then +inf, each by rising class."""
     g = _check_logits(logits, class_dim, temperature)
     if label is not None:
         _check_rows(label, "label", g, torch.int64, logits.device)
@@ -311,7 +313,7 @@ def distill_loss(logits, top_ids, top_logits, temperature=1.0, tail=False, weigh
     softmax(top_logits / temperature) over its entries.  tail=True: top_logits are log probabilities AT `temperature` (class_logprobs(...,
     temperature=temperature)); what they leave of 1 is one more class, against the student's mass outside the entries.
     A negative id is an absent entry, a row without entries counts with loss 0; an id that is no class makes the loss NaN.
-    weight: fp32 per row; rows of weight 0 are not read.  reduction: "mean" (over the weights' sum; NaN where that is 0), "sum", "none"."""
+    weight: fp32 per row; rows of weight 0 are void, whatever they hold.  reduction: "mean" (over the weights' sum; NaN where that is 0), "sum", "none"."""
     g, teacher = _check_distill(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum", "none"))
     if logits.requires_grad and torch.is_grad_enabled():
         return _Distill.apply(logits, g, teacher, float(temperature), bool(tail), reduction)
@@ -323,7 +325,8 @@ def distill_loss_grad(logits, top_ids, top_logits, temperature=1.0, tail=False, 
                       grad_scale=1.0, out=None, accumulate=False):
     """(loss, grad_scale * gradient of the loss) in one call, outside autograd: what a training step that writes its own gradients uses.
     out: the tensor the gradient is written to (logits' shape and type; classes or pixels contiguous as in the logits), added to with
-    accumulate=True; the default is a new one.  The loss itself is not scaled."""
+    accumulate=True; the default is a new one.  Its values may share memory neither with an input nor with each other.  The loss itself
+    is not scaled."""
     g, teacher = _check_distill(logits, top_ids, top_logits, temperature, weight, class_dim, reduction, ("mean", "sum"))
     dev = logits.device
     if out is None:

@@ -265,7 +265,7 @@ class BNL:
 
 # HIP streams (and the split-K scratch arenas that go with them) are shared by every engine of a process, per device.
 # The runtime multiplexes streams onto a handful of hardware queues round-robin: when each engine created its own
-# side / high-priority streams, the streams of the SECOND engine of a process (another input shape, an eval engine, the
+# side / backward-chain streams, the streams of the SECOND engine of a process (another input shape, an eval engine, the
 # module path after the Trainer in bench.py) could land on one hardware queue, and its backward lost the concurrency
 # of the weight-gradient stream with the dependent chain (measured: 207 ms for the first engine of a process, 221-230
 # ms for an identical second one).  Engines of one process never run concurrently, so sharing is safe.
@@ -339,7 +339,7 @@ class Engine:
         # Every weight gradient runs on the side stream (not only the small grids): the direct-to-LDS weight-gradient
         # kernel leaves >= 60 % of the VGPR file and 32 KB of LDS per CU free, so the HBM-bound BatchNorm backward
         # kernels and the data-gradient GEMMs of the main stream are co-resident with it instead of running alone
-        # (measured bs 16: 217.4 -> 207.9 ms per step together with the high-priority chain below, 214.5 without
+        # (measured bs 16, the chain below then still at a raised priority: 217.4 -> 207.9 ms per step together with it, 214.5 without
         # the side stream; scripts/step_variants.py).
         self.side_all = True
         # The dependent chain of backward (data gradients + BatchNorm) runs on a stream of its own beside the side stream of the
@@ -818,7 +818,7 @@ class Engine:
                     lru.append(lru.pop(i))
                 return t
         # at most MAX_SCRATCH_ARENAS (256 MB each) are kept: the streams the engines themselves use (the caller's, the
-        # high-priority chain) plus a few caller streams; the least recently used one is released after a device
+        # backward chain's) plus a few caller streams; the least recently used one is released after a device
         # synchronisation (nothing can still be reading it)
         if len(lru) >= MAX_SCRATCH_ARENAS:
             torch.cuda.synchronize(self.device)

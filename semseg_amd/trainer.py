@@ -155,7 +155,10 @@ class Trainer:
         """x [N,3,H,W] fp32 cuda, y [N,h,w] int64 cuda (per-rank shard).  Returns (pred, main, aux).
 
         top: a teacher's top classes of the score map, (ids, values) or (ids, values, weight) as distill_loss takes them ([N,k,h',w'];
-        HipSegModule.top_logits): adds distill_weight * distillation to the loss, and its value (unweighted) to what is returned."""
+        HipSegModule.top_logits): adds distill_weight * distillation to the loss, and its value (unweighted) to what is returned.  With
+        several ranks the distillation's mean is each rank's own, over its own weights, as the cross entropy's is over its own pixels.
+        distill_weight, distill_temperature, distill_tail and the entries' shape are part of a recorded step: a step that changes one of
+        them, or leaves the teacher out, runs launch by launch and is recorded anew."""
         lr = self.base_lr if lr is None else lr
         # the parameters must still be views of flat_w (model.to()/half()/load_state_dict(assign=True) break that
         # silently: SGD would then update a buffer nobody reads)
